@@ -116,7 +116,10 @@ class NPairLossConfig:
 
 @dataclass
 class SolverConfig:
-    """The SolverParameter subset of usage/solver.prototxt:1-17."""
+    """The SolverParameter subset of usage/solver.prototxt:1-17, and what AdamW
+    adds to it: `type: "AdamW"` takes momentum and momentum2 for its betas, delta
+    for its eps, weight_decay as the decoupled one, and holds its moments in
+    state_bits (32 or 8).  Every other type is SGD, as it always was."""
 
     net: Optional[str] = None
     test_iter: int = 0
@@ -137,6 +140,10 @@ class SolverConfig:
     snapshot_prefix: str = ""
     solver_mode: str = "GPU"
     random_seed: Optional[int] = None
+    type: str = "SGD"
+    momentum2: float = 0.999
+    delta: float = 1e-8
+    state_bits: int = 32
 
     @classmethod
     def from_message(cls, msg: Message) -> "SolverConfig":

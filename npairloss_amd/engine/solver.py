@@ -11,11 +11,12 @@ every 10k iterations), so CaffeSGD implements the Caffe rule exactly.
 
 from __future__ import annotations
 
-from typing import Iterable
+from typing import Iterable, Union
 
 import torch
 
 from ..config.params import SolverConfig
+from .adamw import AdamW
 
 
 class CaffeSGD(torch.optim.Optimizer):
@@ -77,7 +78,13 @@ class CaffeSGD(torch.optim.Optimizer):
 
 
 def build_optimizer(model: torch.nn.Module, solver: SolverConfig,
-                    master_weights: bool = False) -> CaffeSGD:
+                    master_weights: bool = False) -> Union[CaffeSGD, AdamW]:
+    """The solver's optimizer: AdamW where its type says so (momentum and
+    momentum2 are the betas, delta the eps), Caffe's SGD otherwise."""
+    if str(solver.type).lower() == "adamw":
+        return AdamW(model.parameters(), lr=solver.base_lr, betas=(solver.momentum, solver.momentum2),
+                     eps=solver.delta, weight_decay=solver.weight_decay, master_weights=master_weights,
+                     state_bits=solver.state_bits, seed=solver.random_seed or 0)
     return CaffeSGD(model.parameters(), lr=solver.base_lr,
                     momentum=solver.momentum, weight_decay=solver.weight_decay,
                     master_weights=master_weights)

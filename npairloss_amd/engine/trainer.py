@@ -25,7 +25,7 @@ from ..config.params import SolverConfig
 from ..ops.npair_loss import NPairMultiClassLoss
 from ..parallel import collectives as comm
 from ..parallel.ddp import BucketedGradReducer
-from .solver import build_optimizer
+from .solver import CaffeSGD, build_optimizer
 
 
 class AverageWindow:
@@ -121,6 +121,7 @@ class Trainer:
         `<prefix>iter_N.solverstate` (iter + SGD momentum history in
         canonical learnable-parameter order), like the reference solver
         (usage/solver.prototxt:15-16)."""
+        self._need_sgd()
         if comm.rank() != 0:
             return None
         from ..utils.caffemodel import (CaffeSolverState, caffe_param_order,
@@ -149,6 +150,7 @@ class Trainer:
         """Resume mid-training from Caffe artifacts: weights from the
         .caffemodel (name-matched), iteration + SGD momentum from the
         .solverstate (canonical parameter order)."""
+        self._need_sgd()
         from ..utils.caffemodel import (caffe_param_order, load_caffemodel_into,
                                         read_solverstate)
 
@@ -179,6 +181,11 @@ class Trainer:
                 stp["v"] = t
         self.iter = st.iter
         self._graph_state = None  # state tensors replaced: recapture
+
+    def _need_sgd(self):
+        if not isinstance(self.optimizer, CaffeSGD):
+            raise RuntimeError("a .solverstate holds SGD's momentum: use snapshot() and restore() "
+                               f"with {type(self.optimizer).__name__}")
 
     # -- one training iteration --------------------------------------------
 

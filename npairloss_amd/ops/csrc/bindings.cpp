@@ -62,6 +62,25 @@ torch::Tensor sim_gemm_nt(torch::Tensor F_l, torch::Tensor F_g);
 torch::Tensor gemm_nn(torch::Tensor A, torch::Tensor B);
 torch::Tensor gemm_tn(torch::Tensor A, torch::Tensor B);
 
+// rms_norm.hip
+std::vector<torch::Tensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight,
+                                        c10::optional<torch::Tensor> residual, double eps,
+                                        int64_t group);
+std::vector<torch::Tensor> rms_norm_bwd(torch::Tensor dy, c10::optional<torch::Tensor> dsum,
+                                        torch::Tensor s, torch::Tensor weight, torch::Tensor inv);
+
+// rotary.hip
+std::vector<torch::Tensor> rotary_turn(torch::Tensor q, c10::optional<torch::Tensor> k,
+                                       torch::Tensor positions, torch::Tensor frequencies,
+                                       bool interleaved, double amplitude, bool backward);
+
+// adamw.hip
+void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> grads,
+                  std::vector<torch::Tensor> ms, std::vector<torch::Tensor> vs,
+                  std::vector<torch::Tensor> steps, std::vector<torch::Tensor> masters,
+                  std::vector<torch::Tensor> scales, double lr, double b1, double b2, double eps,
+                  double weight_decay, int64_t seed);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "npairloss_amd gfx950 HIP kernels";
   m.def("rowstats", &rowstats, "per-query min_within/max_between/max_all");
@@ -86,5 +105,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused 1x1-conv GEMM + bias + relu (bf16 MFMA)");
   m.def("conv1x1_dgrad", &conv1x1_dgrad, "1x1-conv data gradient GEMM (bf16 MFMA)");
   m.def("gemm_nn", &gemm_nn, "fp32 MFMA GEMM A @ B");
+  m.def("rms_norm_fwd", &rms_norm_fwd, "residual + RMS norm, in the input's type or e4m3");
+  m.def("rms_norm_bwd", &rms_norm_bwd, "RMS norm gradients");
+  m.def("rotary_turn", &rotary_turn, "rotary positions for q and k");
+  m.def("adamw_update", &adamw_update, "AdamW step over many tensors, fp32 or 8-bit moments");
   m.def("gemm_tn", &gemm_tn, "fp32 MFMA GEMM A^T @ B");
 }

@@ -11,6 +11,7 @@ Usage:  python setup.py build_ext --inplace   (or just: python setup.py)
 """
 
 import concurrent.futures
+import glob
 import os
 import shutil
 import subprocess
@@ -33,6 +34,9 @@ SOURCES = [
     "gemm_lowp.hip",
     "biasrelu.hip",
     "conv1x1.hip",
+    "rms_norm.hip",
+    "rotary.hip",
+    "adamw.hip",
 ]
 
 
@@ -68,18 +72,20 @@ def compile_flags(tdir):
         "-O3",
         f"--offload-arch={ARCH}",
         "-fno-gpu-rdc",
+        # no packed fp32 arithmetic: some of its forms give wrong results on this part
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     ]
 
 
 def needs_build(src, obj):
     if not os.path.exists(obj):
         return True
-    dep = [src, os.path.join(CSRC, "common.h"), os.path.abspath(__file__)]
+    dep = [src, os.path.abspath(__file__)] + glob.glob(os.path.join(CSRC, "*.h"))
     omt = os.path.getmtime(obj)
     return any(os.path.getmtime(d) > omt for d in dep if os.path.exists(d))
 
 
-def build(verbose=True):
+def build(verbose=True, force=False):
     os.makedirs(BUILD, exist_ok=True)
     tdir = torch_paths()
     flags = compile_flags(tdir)
@@ -90,7 +96,7 @@ def build(verbose=True):
         sp = os.path.join(CSRC, src)
         op = os.path.join(BUILD, src.replace("/", "_") + ".o")
         objs.append(op)
-        if needs_build(sp, op):
+        if force or needs_build(sp, op):
             jobs.append((sp, op))
 
     def compile_one(sp_op):
