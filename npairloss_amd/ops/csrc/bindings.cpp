@@ -81,6 +81,17 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
                   std::vector<torch::Tensor> scales, double lr, double b1, double b2, double eps,
                   double weight_decay, int64_t seed);
 
+// attention.hip
+std::vector<torch::Tensor> attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double softcap,
+                                         c10::optional<torch::Tensor> slopes, bool causal,
+                                         c10::optional<torch::Tensor> prefix, c10::optional<torch::Tensor> q_doc,
+                                         c10::optional<torch::Tensor> k_doc);
+std::vector<torch::Tensor> attention_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                         torch::Tensor o, torch::Tensor lse, double scale, double softcap,
+                                         c10::optional<torch::Tensor> slopes, bool causal,
+                                         c10::optional<torch::Tensor> prefix, c10::optional<torch::Tensor> q_doc,
+                                         c10::optional<torch::Tensor> k_doc);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "npairloss_amd gfx950 HIP kernels";
   m.def("rowstats", &rowstats, "per-query min_within/max_between/max_all");
@@ -109,5 +120,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm_bwd", &rms_norm_bwd, "RMS norm gradients");
   m.def("rotary_turn", &rotary_turn, "rotary positions for q and k");
   m.def("adamw_update", &adamw_update, "AdamW step over many tensors, fp32 or 8-bit moments");
+  m.def("attention_fwd", &attention_fwd, "masked attention forward");
+  m.def("attention_bwd", &attention_bwd, "masked attention gradients");
   m.def("gemm_tn", &gemm_tn, "fp32 MFMA GEMM A^T @ B");
 }

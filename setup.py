@@ -37,6 +37,7 @@ SOURCES = [
     "rms_norm.hip",
     "rotary.hip",
     "adamw.hip",
+    "attention.hip",
 ]
 
 

@@ -1,0 +1,310 @@
+"""attention against the formula in 64 bits: masks, heads, lengths, types, strides,
+gradients, rows that see nothing, and values that nobody sees."""
+
+import math
+
+import pytest
+import torch
+
+from npairloss_amd.ops import attention
+from transformer_util import DEVICES, TYPES, U, assert_within, half_step, least, replays
+
+
+def case(B=2, Lq=5, Lk=None, H=2, Hk=None, D=16, softcap=0.0, slopes=False, causal=False, prefix=None, documents=None, scale=None):
+    Lk, Hk = Lk or Lq, Hk or H
+    return dict(B=B, Lq=Lq, Lk=Lk, H=H, Hk=Hk, D=D, softcap=softcap, slopes=slopes, causal=causal, prefix=prefix, documents=documents, scale=scale)
+
+
+CASES = {
+    "one": case(B=1, Lq=1, H=1, D=8),
+    "one of few": case(Lq=1, Lk=7, H=4, Hk=2, D=64),
+    "plain": case(Lq=197, H=3, D=64),
+    "odd width": case(Lq=40, H=2, D=20),
+    "width 80": case(Lq=65, H=2, D=80, softcap=5.0),
+    "width 128": case(Lq=130, H=4, Hk=1, D=128),
+    "width 1": case(Lq=9, H=1, D=1),
+    "causal": case(Lq=70, H=2, D=32, causal=True),
+    "causal, more keys": case(Lq=33, Lk=150, H=4, Hk=2, D=64, causal=True, slopes=True),
+    "causal, more queries": case(Lq=90, Lk=31, H=2, D=64, causal=True),
+    "prefix": case(B=3, Lq=100, H=2, D=64, causal=True, prefix=[0, 64, 100]),
+    "capped": case(Lq=64, H=2, D=64, softcap=3.0),
+    "slopes": case(Lq=129, H=6, Hk=3, D=64, slopes=True),
+    "documents": case(Lq=200, H=2, D=64, documents="packed"),
+    "documents, mixed": case(Lq=150, H=2, Hk=1, D=64, documents="mixed", softcap=10.0),
+    "documents, one query": case(B=5, Lq=1, Lk=300, H=8, Hk=2, D=128, documents="lengths"),
+    "documents, causal": case(Lq=131, H=2, D=32, documents="packed", causal=True, slopes=True),
+    "all padding": case(Lq=20, H=2, D=16, documents="padding"),
+    "few queries, long": case(B=1, Lq=3, Lk=1500, H=4, Hk=1, D=64, causal=True, softcap=20.0),
+    "two tiles": case(B=1, Lq=128, H=1, D=128, scale=0.3),
+    "uneven": case(B=1, Lq=257, Lk=383, H=2, D=96, causal=True, prefix=[300], slopes=True),
+}
+
+
+def inputs(c, dtype, device, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    normal = lambda *s: torch.randn(*s, generator=g).to(dtype).to(device)  # noqa: E731
+    q, k, v = normal(c["B"], c["Lq"], c["H"], c["D"]), normal(c["B"], c["Lk"], c["Hk"], c["D"]), normal(c["B"], c["Lk"], c["Hk"], c["D"])
+    dout = normal(c["B"], c["Lq"], c["H"], c["D"])
+    more = dict(softcap=c["softcap"], causal=c["causal"], scale=c["scale"])
+    if c["slopes"]:
+        more["slopes"] = torch.tensor([2.0 ** -(h + 1) for h in range(c["H"])], device=device)
+    if c["prefix"] is not None:
+        more["prefix"] = torch.tensor(c["prefix"], dtype=torch.int32, device=device)
+    if c["documents"] == "packed":  # pieces in a row, padding behind
+        ids = torch.full((c["B"], c["Lk"]), -1, dtype=torch.int32)
+        for b in range(c["B"]):
+            at, n = 0, 0
+            while at < c["Lk"] - 10:
+                step = int(torch.randint(1, 90, (1,), generator=g))
+                ids[b, at:min(at + step, c["Lk"] - 10)] = n
+                at, n = at + step, n + 1
+        more["documents"] = ids.to(device)
+    elif c["documents"] == "mixed":  # in no order
+        more["documents"] = torch.randint(-1, 4, (c["B"], c["Lk"]), generator=g, dtype=torch.int32).to(device)
+    elif c["documents"] == "lengths":
+        ids = torch.zeros(c["B"], c["Lk"], dtype=torch.int32)
+        for b in range(c["B"]):
+            ids[b, [0, 1, 63, 64, 299][b]:] = -1
+        more["documents"], more["key_documents"] = torch.zeros(c["B"], c["Lq"], dtype=torch.int32, device=device), ids.to(device)
+    elif c["documents"] == "padding":
+        more["documents"] = torch.full((c["B"], c["Lk"]), -1, dtype=torch.int32, device=device)
+    return q, k, v, dout, more
+
+
+def mask_of(more, B, Lq, Lk):
+    at, j = torch.arange(Lq)[:, None] + (Lk - Lq), torch.arange(Lk)[None]
+    seen = torch.ones(B, Lq, Lk, dtype=torch.bool)
+    if more.get("causal"):
+        seen = (j <= at).expand(B, Lq, Lk)
+        if more.get("prefix") is not None:
+            seen = seen | (j < more["prefix"].cpu()[:, None, None])
+    if more.get("documents") is not None:
+        d = more["documents"].cpu()
+        kd = more.get("key_documents", more["documents"]).cpu()
+        seen = seen & (d[:, :, None] == kd[:, None, :]) & (kd[:, None, :] >= 0)
+    return seen[:, None], (at - j).abs()
+
+
+def exact(q, k, v, dout, more, dtype):
+    """Outputs, gradients and what each may be off by."""
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    G = H // Hk
+    qf, kf, vf, gf = (x.detach().double().cpu().transpose(1, 2) for x in (q, k, v, dout))
+    kf, vf = (x.repeat_interleave(G, 1) for x in (kf, vf))
+    scale = more.get("scale") or D ** -0.5
+    cap = more.get("softcap", 0.0)
+    seen, distance = mask_of(more, B, Lq, Lk)
+    raw = qf @ kf.transpose(2, 3) * scale
+    # scores: the product's sum (each of D products and sums one unit of the magnitudes), the scale, the bias, log2(e);
+    # the cap: tanh from an exponential of up to 2 |s / cap| and a quotient, 8 units of cap
+    error = qf.abs() @ kf.abs().transpose(2, 3) * scale * (D + 4) * U
+    bend = torch.ones_like(raw)
+    if cap:
+        t = torch.tanh(raw / cap)
+        raw, bend = cap * t, 1 - t * t
+        error = error + cap * 8 * U + raw.abs() * 4 * U
+    if more.get("slopes") is not None:
+        bias = more["slopes"].double().cpu().view(-1, 1, 1) * distance
+        raw, error = raw - bias, error + (raw.abs() + bias) * 4 * U
+    s = raw.masked_fill(~seen, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    none = ~seen.any(-1, keepdim=True)
+    p = torch.where(seen, torch.exp(s - torch.where(none, 0.0, top)), 0.0)
+    p = torch.where(none, 0.0, p / p.sum(-1, keepdim=True).clamp_min(1e-300))
+    o = p @ vf
+    # the exponent's argument in base 2 is rounded (|s - top| and |s| units), numerator and denominator alike
+    spread = torch.where(seen, error + (raw.abs() + (raw - torch.where(none, 0.0, top)).abs()) * 4 * U, 0.0)
+    rel = 2 * spread.amax(-1, keepdim=True) + 2 * spread + (Lk + 16) * U  # of a weight
+    e = half_step(dtype)
+    pe = e if dtype != torch.float32 else 0.0                       # weights rounded to the type
+    tiny = least(dtype) if dtype == torch.float16 else 0.0          # fp16: and to its least step
+    err_o = (p * (rel + pe) + tiny * seen) @ vf.abs() + o.abs() * 8 * U
+    tol = {"out": err_o + o.abs() * e + least(dtype)}
+    want = {"out": o}
+    o_r, delta_e = o, (gf.abs() * (err_o + o.abs() * e + least(dtype))).sum(-1, keepdim=True) + (gf * o).abs().sum(-1, keepdim=True) * (D + 2) * U
+    dp = gf @ vf.transpose(2, 3)
+    delta = (gf * o_r).sum(-1, keepdim=True)
+    ds = p * (dp - delta) * scale * bend
+    bend_e = 0.0 if not cap else p * (dp - delta).abs() * scale * (16 * U + 2 * error / cap)
+    err_ds = ds.abs() * (rel + 2 * pe + 8 * U) + p * scale * bend.abs() * (gf.abs() @ vf.abs().transpose(2, 3) * (D + 4) * U + delta_e) + bend_e
+    err_ds = torch.where(seen, err_ds + tiny * scale, 0.0)
+    err_p = torch.where(seen, p * (rel + pe) + tiny, 0.0)
+    ds = torch.where(seen, ds, 0.0)
+    n = lambda x: x.transpose(2, 3)  # noqa: E731
+    fold = lambda x: x.view(B, Hk, G, Lk, D).sum(2)  # noqa: E731
+    got = {"dq": (ds @ kf, err_ds @ kf.abs() + ds.abs() @ kf.abs() * (Lk + 8) * U),
+           "dk": (fold(n(ds) @ qf), fold(n(err_ds) @ qf.abs() + n(ds.abs()) @ qf.abs() * (Lq * G + 8) * U)),
+           "dv": (fold(n(p) @ gf), fold(n(err_p) @ gf.abs() + n(p) @ gf.abs() * (Lq * G + 8) * U))}
+    for name, (x, err) in got.items():
+        want[name], tol[name] = x, err + x.abs() * e + least(dtype)
+    return {a: x.transpose(1, 2) for a, x in want.items()}, {a: x.transpose(1, 2) for a, x in tol.items()}
+
+
+def run(q, k, v, dout, more):
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    o = attention(q, k, v, **more)
+    return dict(zip(("out", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, (q, k, v), dout)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", CASES)
+def test_formula(name, dtype, device):
+    q, k, v, dout, more = inputs(CASES[name], dtype, device)
+    got = run(q, k, v, dout, more)
+    want, tol = exact(q, k, v, dout, more, dtype)
+    for n in want:
+        assert got[n].dtype == dtype
+        assert_within(got[n], want[n], tol[n], n)
+    with torch.no_grad():
+        assert torch.equal(attention(q, k, v, **more), got["out"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", ["capped", "documents, causal", "causal, more keys"])
+def test_gradient_against_differences(name, device):
+    q, k, v, dout, more = inputs(CASES[name], torch.float32, device, seed=2)
+    got = run(q, k, v, dout, more)
+    _, tol = exact(q, k, v, dout, more, torch.float32)
+    g = torch.Generator().manual_seed(1)
+    at = {n: x.double().cpu() for n, x in (("dq", q), ("dk", k), ("dv", v))}
+
+    def loss(at):
+        want, _ = exact(at["dq"], at["dk"], at["dv"], dout, more, torch.float32)
+        return float((want["out"] * dout.double().cpu()).sum())
+
+    for n in at:
+        u = torch.randn(at[n].shape, generator=g).double()
+        h = 1e-5
+        fd = (loss({**at, n: at[n] + h * u}) - loss({**at, n: at[n] - h * u})) / (2 * h)
+        mine = float((got[n].double().cpu() * u).sum())
+        # the gradient's own tolerance, and the differences' h^2 and 10^-16 / h
+        assert abs(fd - mine) <= float((tol[n] * u.abs()).sum()) + 1e-6 * (1 + abs(fd)), (n, fd, mine)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["causal, more keys", "documents", "documents, mixed", "documents, one query", "prefix", "few queries, long", "uneven"])
+def test_what_nobody_sees(name, dtype, device):
+    """NaN and infinities in keys, values, queries and gradients of other documents and
+    of padding: everything else is as if they were not there."""
+    q, k, v, dout, more = inputs(CASES[name], dtype, device)
+    B, Lq, Lk = q.shape[0], q.shape[1], k.shape[1]
+    seen = mask_of(more, B, Lq, Lk)[0][:, 0]
+    bad_k, bad_q = torch.zeros(B, Lk, dtype=torch.bool), torch.zeros(B, Lq, dtype=torch.bool)
+    if more.get("documents") is not None:
+        kd, qd = more.get("key_documents", more["documents"]).cpu(), more["documents"].cpu()
+        bad_k, bad_q = (kd < 0) | (kd == 1), (qd < 0) | (qd == 1)
+    else:
+        bad_k[:, Lk - 3:] = True  # seen by the last queries alone
+        bad_q = (seen & bad_k[:, None]).any(-1)
+    clean = run(q, k, v, dout, more)
+    want, tol = exact(q, k, v, dout, more, dtype)
+    q, k, v, dout = (x.clone() for x in (q, k, v, dout))
+    for x, bad in ((q, bad_q), (k, bad_k), (v, bad_k), (dout, bad_q)):
+        bad = bad.to(device)
+        x[bad] = torch.tensor([math.nan, math.inf, -math.inf, 1.0], device=device).repeat(-(-x[bad].numel() // 4))[:x[bad].numel()].view(x[bad].shape).to(dtype)
+    got = run(q, k, v, dout, more)
+    fine_q, fine_k = ~bad_q, ~bad_k & ~(seen & bad_q[..., None]).any(1)
+    for n, fine in (("out", fine_q), ("dq", fine_q), ("dk", fine_k), ("dv", fine_k)):
+        fine = fine.to(device)
+        assert_within(got[n][fine], want[n][fine.cpu()], tol[n][fine.cpu()], n)
+        assert clean[n][fine].isfinite().all()
+    none = ~seen.any(-1).to(device)
+    assert (got["out"][none] == 0).all() and (got["dq"][none] == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_not_finite_where_it_is_seen(device):
+    q, k, v, dout, more = inputs(CASES["plain"], torch.float32, device)
+    v[0, 3, 1, 2] = math.nan
+    k[1, 5, 0, 0] = math.nan
+    o = attention(q, k, v)
+    bad = torch.zeros(o.shape, dtype=torch.bool)
+    bad[0, :, 1, 2] = True
+    bad[1, :, 0] = True
+    assert torch.equal(o.isnan().cpu(), bad)
+    q, k, v, dout, more = inputs(CASES["causal"], torch.float32, device)
+    v[0, 40, 0, 1] = math.inf
+    o = attention(q, k, v, causal=True)
+    bad = torch.zeros(o.shape, dtype=torch.bool)
+    bad[0, 40:, 0, 1] = True
+    assert torch.equal((o == math.inf).cpu(), bad) and o.cpu()[~bad].isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides(dtype, device):
+    """Views of a packed projection, heads first, elements apart, rows off the border, a broadcast gradient."""
+    g = torch.Generator().manual_seed(7)
+    qkv = torch.randn(2, 50, 8, 32, generator=g).to(dtype).to(device)
+    q, k, v = qkv[:, :, :4], qkv[:, :, 4:6], qkv[:, :, 6:]
+    dout = torch.randn(2, 50, 4, 32, generator=g).to(dtype).to(device)
+    base = run(*(x.contiguous() for x in (q, k, v, dout)), dict(causal=True))
+    heads = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    apart = lambda x: torch.stack([x, x], -1)[..., 0]  # noqa: E731
+    off = lambda x: torch.cat([x.flatten()[:1], x.flatten()])[1:].view(x.shape)  # noqa: E731
+    for how in (lambda x: x, heads, apart, off):
+        got = run(how(q), how(k), how(v), how(dout), dict(causal=True))
+        assert all(torch.equal(got[n], base[n]) for n in base)
+    one = torch.ones((), dtype=dtype, device=device).expand(dout.shape)
+    got, base = run(q, k, v, one, {}), run(q, k, v, one.contiguous(), {})
+    assert all(torch.equal(got[n], base[n]) for n in base)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_empty(device):
+    for B, Lq, Lk, H in ((0, 3, 3, 2), (2, 0, 3, 2), (2, 3, 0, 2), (2, 0, 0, 2)):
+        q, k = torch.randn(B, Lq, H, 16, device=device, requires_grad=True), torch.randn(B, Lk, H, 16, device=device, requires_grad=True)
+        o = attention(q, k, k)
+        assert o.shape == (B, Lq, H, 16) and (o == 0).all()
+        o.sum().backward()
+        assert (q.grad == 0).all() and (k.grad == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    q, k = torch.randn(2, 4, 4, 16, device=device), torch.randn(2, 6, 2, 16, device=device)
+    ids = lambda *s: torch.zeros(*s, dtype=torch.int32, device=device)  # noqa: E731
+    slopes = torch.ones(4, device=device)
+    for kind, args, more in [
+            (ValueError, (q[0], k, k), {}), (TypeError, (q.double(), k.double(), k.double()), {}), (TypeError, (q, k.half(), k.half()), {}),
+            (ValueError, (q, k, k[:, :5]), {}), (ValueError, (q, k[:1], k[:1]), {}), (ValueError, (q, k[..., :8], k[..., :8]), {}),
+            (ValueError, (q[:, :, :3], k, k), {}), (ValueError, (q, k[:, :, :0], k[:, :, :0]), {}), (ValueError, (q, k, k), dict(softcap=-1.0)),
+            (ValueError, (q, k, k), dict(softcap=math.inf)), (ValueError, (q, k, k), dict(scale=math.nan)), (ValueError, (q, k, k), dict(slopes=slopes[:3])),
+            (ValueError, (q, k, k), dict(slopes=slopes.half())), (RuntimeError, (q, k, k), dict(slopes=slopes.clone().requires_grad_())),
+            (ValueError, (q, k, k), dict(prefix=ids(2))), (ValueError, (q, k, k), dict(causal=True, prefix=ids(3))),
+            (ValueError, (q, k, k), dict(causal=True, prefix=ids(2).long())), (ValueError, (q, k, k), dict(documents=ids(2, 4))),
+            (ValueError, (q, k, k), dict(key_documents=ids(2, 6))), (ValueError, (q, k, k), dict(documents=ids(2, 4), key_documents=ids(2, 5))),
+            (ValueError, (q, k, k), dict(documents=ids(2, 4).long(), key_documents=ids(2, 6)))]:
+        with pytest.raises(kind):
+            attention(*args, **more)
+    wide = torch.randn(1, 2, 1, 129, device=device)
+    with pytest.raises(ValueError):
+        attention(wide, wide, wide)
+
+
+@pytest.mark.gpu
+def test_captured():
+    """Forward and backward replayed; two graphs of one call do not share their workspaces' contents."""
+    q, k, v, dout, more = inputs(CASES["documents, causal"], torch.bfloat16, "cuda")
+    want = run(q, k, v, dout, more)
+    for out in replays(lambda: run(q, k, v, dout, more)):
+        assert all(torch.equal(out[n], want[n]) for n in want)
+    one = inputs(CASES["documents, one query"], torch.bfloat16, "cuda")
+    alone = attention(*one[:3], **one[4])
+    for out in replays(lambda: attention(*one[:3], **one[4])):
+        assert torch.equal(out, alone)
+
+
+@pytest.mark.gpu
+def test_repeated_and_on_another_stream():
+    q, k, v, dout, more = inputs(case(B=2, Lq=700, H=4, Hk=2, D=64, causal=True), torch.bfloat16, "cuda")
+    first = run(q, k, v, dout, more)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = run(q, k, v, dout, more)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(first[n], again[n]) for n in first)
