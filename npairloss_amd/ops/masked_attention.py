@@ -109,7 +109,8 @@ def _ready(x, width):
     if x.shape[-1] != width:
         return torch.nn.functional.pad(x, (0, width - x.shape[-1]))
     per16 = 16 // x.element_size()
-    if x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % per16 for s in x.stride()[:3]):
+    far = x.shape[1] > 1 and x.stride(1) * x.element_size() > 1 << 24  # offsets within a tile are 32 bits
+    if x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % per16 for s in x.stride()[:3]) or far:
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
