@@ -21,6 +21,7 @@ struct AttnArgs {
   const void* q; const void* k; const void* v;
   RowStrides qs, ks, vs;
   void* o;               // [B, Lq, H, D]
+  void* o_rest;          // [B, Lq, H, D] or null: what rounding took from o, for delta
   float* lse;            // [B, H, Lq]
   int B, Lq, Lk, H, Hk, D;
   float scale;
@@ -33,6 +34,7 @@ struct AttnArgs {
   // backward
   const void* dout; RowStrides gs;
   const float* delta;    // [B, H, Lq]: sum_d dout o
+  const unsigned* grad_top;  // bits of the largest |dout| (fp16) or null
   void* dq;              // [B, Lq, H, D]
   void* dk; void* dv;    // [B, Lk, Hk, D]
 };
@@ -45,13 +47,14 @@ DEVINL int causal_end(const AttnArgs& a, int b, int i) {
 
 DEVINL bool seen_by_documents(int dq, int dk) { return dq == dk && dk >= 0; }
 
-// Exact to a few units where the type's own rounding is far coarser; fp32 takes
-// the library's.
-template <typename T> DEVINL float tanh_of(float x) {
-  const float e = __builtin_amdgcn_exp2f(2.f * kLog2e * fabsf(x));
-  return copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f), x);
+// The cap as c tanh(s / c) = c - 2 c u with u = 1 / (1 + 2^(2 log2(e) s / c)), and its
+// derivative 1 - tanh^2 = 4 u (1 - u): an exponential and a reciprocal, each a unit
+// or so off, under 8 units of c together.  fp32 takes the library's exponential and
+// a true quotient.
+template <typename T> DEVINL float cap_share(float s_over_c) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * s_over_c));
 }
-template <> DEVINL float tanh_of<float>(float x) { return tanhf(x); }
+template <> DEVINL float cap_share<float>(float s_over_c) { return 1.f / (1.f + expf(2.f * s_over_c)); }
 
 template <typename T>
 DEVINL float dot_row(const T* __restrict__ x, const T* __restrict__ y, int D) {
@@ -72,9 +75,9 @@ DEVINL float transformed(const AttnArgs& a, float dot, float slope, int distance
   float s = dot * a.scale;
   *bend = 1.f;
   if (a.softcap > 0.f) {
-    const float t = tanh_of<T>(s / a.softcap);
-    s = a.softcap * t;
-    *bend = 1.f - t * t;
+    const float u = cap_share<T>(s / a.softcap);
+    s = a.softcap - 2.f * a.softcap * u;
+    *bend = 4.f * u * (1.f - u);
   }
   return (s - slope * static_cast<float>(distance)) * kLog2e;
 }
@@ -145,10 +148,16 @@ DEVINL void forward_row(const AttnArgs& a, int b, int i, int h) {
         if (lane + 64 * x < a.D) o[x] += w * to_f(v[lane + 64 * x]);
     }
   }
-  T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D;
+  const int64_t at_o = ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D;
+  T* out = static_cast<T*>(a.o) + at_o;
+  T* rest = static_cast<T*>(a.o_rest) + at_o;
 #pragma unroll
   for (int x = 0; x < 2; ++x)
-    if (lane + 64 * x < a.D) out[lane + 64 * x] = from_f<T>(none ? 0.f : o[x] / total);
+    if (lane + 64 * x < a.D) {
+      const float value = none ? 0.f : o[x] / total;
+      out[lane + 64 * x] = from_f<T>(value);
+      if (a.o_rest != nullptr) rest[lane + 64 * x] = from_f<T>(value - to_f(from_f<T>(value)));
+    }
   if (lane == 0) a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + i] = none ? INFINITY : top + log2f(total);
 }
 

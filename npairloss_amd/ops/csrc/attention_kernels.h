@@ -1,0 +1,1061 @@
+// The attention kernels and how they are launched, for one element type a source
+// file (gfx950).  The mathematics stands in attention.h.
+#pragma once
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+
+#include "attention_tile.h"
+#include "attention_launch.h"
+
+namespace {
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / WAVE;
+constexpr int kQueries = 32 * kWaves;  // of a workgroup of the tiled kernels
+
+// The keys before which the query of a lane sees any (0: none), and its id.
+struct Query {
+  int at, end, doc;
+  float slope2;  // times log2(e)
+};
+
+DEVINL Query query_of(const AttnArgs& a, int b, int i, int h, bool ok) {
+  Query q;
+  q.at = i + a.Lk - a.Lq;
+  q.doc = ok && a.q_doc != nullptr ? a.q_doc[static_cast<int64_t>(b) * a.Lq + i] : 0;
+  q.end = !ok || q.doc < 0 ? 0 : a.causal ? max(0, min(a.Lk, causal_end(a, b, i))) : a.Lk;
+  q.slope2 = ok && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
+  return q;
+}
+
+// What scores go through, as a constant of the kernel, so that products and
+// exponentials are one block of instructions: nothing (one factor, not zero); the
+// cap; a bias with or without the cap, or a factor of zero.
+enum Score { kPlain, kCapped, kBiased };
+
+// Scores in registers to base-2 scores: on return a score is s * (the returned
+// factor).  Lanes are queries and registers keys: `first` is the key of register 0
+// of half 0.  `bend`: the cap's derivative, for the backward pass.
+template <typename T, Score SC, bool BEND>
+DEVINL float transform(const AttnArgs& a, f32x16& s, f32x16* bend, int first, int at, float slope2) {
+  const float c = fabsf(a.scale) * kLog2e;
+  if (SC == kPlain) return c;
+  const int half = threadIdx.x % WAVE / 32;
+  if (SC == kCapped || a.softcap > 0.f) {
+    const float in = fabsf(a.scale) / a.softcap, out = a.softcap * kLog2e;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float u = cap_share<T>(s[r] * in);
+      s[r] = fmaf(-2.f * out, u, out);
+      if (BEND) (*bend)[r] = 4.f * fmaf(-u, u, u);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= c;
+  }
+  if (SC == kBiased) {
+    const float d0 = static_cast<float>(at - first - 4 * half);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] -= slope2 * fabsf(d0 - static_cast<float>(result_row(r, 0)));
+  }
+  return 1.f;
+}
+
+// Which registers a query sees, as bits.
+DEVINL uint32_t seen_keys(const AttnArgs& a, const Query& q, const int* kd, int first, int row0) {
+  const int half = threadIdx.x % WAVE / 32, left = q.end - first - 4 * half;
+  uint32_t seen = 0;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) seen |= static_cast<uint32_t>(result_row(r, 0) < left) << r;
+  if (a.k_doc != nullptr) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int4 d = *reinterpret_cast<const int4*>(kd + row0 + 8 * x + 4 * half);
+      const uint32_t same = static_cast<uint32_t>(d.x == q.doc) | static_cast<uint32_t>(d.y == q.doc) << 1 |
+                            static_cast<uint32_t>(d.z == q.doc) << 2 | static_cast<uint32_t>(d.w == q.doc) << 3;
+      seen &= same << (4 * x) | ~(15u << (4 * x));
+    }
+  }
+  return seen;
+}
+
+// --- forward ----------------------------------------------------------------
+
+// The running softmax of 32 queries (a lane and its other half hold one) and
+// their outputs, transposed: columns are queries, rows the width.  `l` is the
+// lane's own part of the sum.  The outputs are scaled at every tile: a branch around
+// that made the compiler keep them twice.
+template <typename T, int DP, int NS>
+struct Online {
+  f32x16 o[DP / 32];
+  float top, l;
+
+  DEVINL void clear() {
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) o[x] = zeros16();
+    top = -INFINITY;
+    l = 0.f;
+  }
+
+  template <Score SC, bool MASKED>
+  DEVINL void absorb(const AttnArgs& a, const Reader<T, DP>& reader, const Frag<T> (&qf)[DP / 16], const T* ks, const T* vs, const int* kd,
+                     const Query& q, int first) {
+    const Reader<T, DP> at = reader.fresh();
+    Frag<T> p[NS][2];
+    f32x16 s[NS];
+    scores(at, qf, ks, s);
+    weights<SC, MASKED>(a, s, p, kd, q, first);
+    outputs(at, vs, p);
+  }
+
+  DEVINL void scores(const Reader<T, DP>& at, const Frag<T> (&qf)[DP / 16], const T* ks, f32x16 (&s)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      s[n] = zeros16();
+#pragma unroll
+      for (int step = 0; step < DP / 16; ++step) product(at.rows(ks, 32 * n, step), qf[step], s[n]);
+    }
+    paced<T, NS * DP / 16, 1, 4>();
+  }
+
+  template <Score SC, bool MASKED>
+  DEVINL void weights(const AttnArgs& a, f32x16 (&s)[NS], Frag<T> (&p)[NS][2], const int* kd, const Query& q, int first) {
+    float c = 1.f, high = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) c = transform<T, SC, false>(a, s[n], nullptr, first + 32 * n, q.at, q.slope2);
+    if (MASKED) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const uint32_t seen = seen_keys(a, q, kd, first + 32 * n, 32 * n);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = (seen >> r & 1) ? s[n][r] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) high = fmaxf(high, s[n][r]);
+    high = fmaxf(high, other_half(high)) * c;
+    const float now = fmaxf(top, high), from = now == -INFINITY ? 0.f : now;
+    const float keep = __builtin_amdgcn_exp2f(top - from);
+    top = now;
+    l *= keep;
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[x][r] *= keep;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -from));
+        l += w;
+        p[n][r / 8].set(r % 8, w);
+      }
+  }
+
+  DEVINL void outputs(const Reader<T, DP>& at, const T* vs, const Frag<T> (&p)[NS][2]) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) product(at.columns(vs, 32 * n + 16 * t, x), p[n][t], o[x]);
+    paced<T, NS * DP / 16, 2, 4>();
+  }
+};
+
+// Four neighbouring elements of a row.
+template <typename T>
+DEVINL void store4(T* p, float a, float b, float c, float d) {
+  struct alignas(4 * sizeof(T)) Four { T v[4]; };
+  *reinterpret_cast<Four*>(p) = Four{{from_f<T>(a), from_f<T>(b), from_f<T>(c), from_f<T>(d)}};
+}
+
+// A lane's column of a transposed result times `by`, to the row at `out`.
+template <typename T, int DP>
+DEVINL void store_column(T* out, const f32x16 (&o)[DP / 32], int D, float by) {
+  const int half = threadIdx.x % WAVE / 32;
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * x + result_row(r, half);
+      if (d < D) store4(out + d, o[x][r] * by, o[x][r + 1] * by, o[x][r + 2] * by, o[x][r + 3] * by);
+    }
+}
+
+// What rounding takes from them.
+template <typename T, int DP>
+DEVINL void store_rest(T* out, const f32x16 (&o)[DP / 32], int D, float by) {
+  const int half = threadIdx.x % WAVE / 32;
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * x + result_row(r, half);
+      float e[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float value = o[x][r + y] * by;
+        e[y] = value - to_f(from_f<T>(value));
+      }
+      if (d < D) store4(out + d, e[0], e[1], e[2], e[3]);
+    }
+}
+
+template <int N>
+DEVINL bool finite_column(const f32x16 (&o)[N]) {
+  bool fine = true;
+#pragma unroll
+  for (int x = 0; x < N; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) fine = fine && fabsf(o[x][r]) <= FLT_MAX;
+  return fine;
+}
+
+// Of 32 columns, which have a value that is not finite in either half.
+DEVINL uint32_t bad_columns(bool bad) {
+  const uint64_t both = __ballot(bad);
+  return static_cast<uint32_t>(both) | static_cast<uint32_t>(both >> 32);
+}
+
+// Rows that come out not finite are done again one by one: a matrix product
+// multiplies what a masked place holds by zero, and NaN or infinity there spoils
+// the sum; an fp16 operand may overflow.  Without masks and in types of fp32's
+// range the value is the formula's own.
+template <typename T>
+DEVINL bool repairs(const AttnArgs& a) { return sizeof(T) == 2 || a.causal || a.k_doc != nullptr; }
+
+template <typename T, int DP, Score SC>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void forward_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
+  constexpr int KT = sizeof(T) == 2 ? 64 : 32, NS = KT / 32;
+  __shared__ __attribute__((aligned(16))) T ks[2][KT * DP];
+  __shared__ __attribute__((aligned(16))) T vs[2][KT * DP];
+  __shared__ __attribute__((aligned(16))) int kd[2][KT];
+  const int t = threadIdx.x, lane = t % WAVE;
+  const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
+  const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
+  const int64_t bh = linear / q_tiles;
+  const int i0 = (q_tiles - 1 - static_cast<int>(linear % q_tiles)) * kQueries;
+  const int b = bh / a.H, h = bh % a.H, kv = h / (a.H / a.Hk);
+  const int i = i0 + 32 * wave + lane % 32;
+  const bool ok = i < a.Lq;
+  const Query q = query_of(a, b, i, h, ok);
+  Frag<T> qf[DP / 16];
+  load_operands<T, DP>(q_row<T>(a, b, ok ? i : 0, h), ok, a.D, qf);
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int x = 0; x < DP / 16; ++x) qf[x].v = -qf[x].v;
+  }
+  // rows that are not there decide nothing, and nothing of them is kept
+  const int least_end = wave_min(ok ? q.end : INT_MAX), most_end = wave_max(q.end);
+  const int doc_lo = wave_min(ok ? q.doc : INT_MAX), doc_hi = wave_max(ok ? q.doc : INT_MIN);
+
+  int lo = 0, hi = 0;  // ids of the workgroup's queries
+  if (ranges != nullptr) {
+    lo = INT_MAX, hi = -1;
+#pragma unroll
+    for (int x = 0; x < kQueries; x += WAVE)
+      if (i0 + x + lane < a.Lq) {
+        const int id = a.q_doc[static_cast<int64_t>(b) * a.Lq + i0 + x + lane];
+        if (id >= 0) lo = min(lo, id);
+        hi = max(hi, id);
+      }
+    lo = wave_min(lo), hi = wave_max(hi);
+  }
+  const int j_end = a.causal ? max(0, min(a.Lk, causal_end(a, b, min(i0 + kQueries, a.Lq) - 1))) : a.Lk;
+  const int k_tiles = (a.Lk + kDocTile - 1) / kDocTile;
+  const DocRange* own = ranges != nullptr ? ranges + static_cast<int64_t>(b) * k_tiles : nullptr;
+  TileWalk walk(own, lo, hi, 0, (j_end + kDocTile - 1) / kDocTile);
+  int rest = -1;  // the second half of a tile of ids where a tile of keys is smaller
+  auto next = [&]() {
+    if (KT < kDocTile && rest >= 0) {
+      const int j = rest;
+      rest = -1;
+      return j;
+    }
+    const int n = walk.next();
+    if (n < 0) return -1;
+    if (KT < kDocTile && n * kDocTile + KT < j_end) rest = n * kDocTile + KT;
+    return n * kDocTile;
+  };
+  const T* k0 = k_row<T>(a, b, 0, kv);
+  const T* v0 = v_row<T>(a, b, 0, kv);
+  const int* d0 = a.k_doc != nullptr ? a.k_doc + static_cast<int64_t>(b) * a.Lk : nullptr;
+
+  const Reader<T, DP> at;
+  Online<T, DP, NS> run;
+  run.clear();
+  uint32_t ids = 0;
+  DocRange range{0, 0, 0}, range_next{0, 0, 0};
+  uint64_t there = 0;
+  auto load = [&](int j, auto buf) {
+    there = first_rows(a.Lk - j);
+    if (own != nullptr) {
+      range_next = own[j / kDocTile];
+      there = range_next.there >> (j % kDocTile);
+      ids = staged_word(d0 + j, t, min(KT, a.Lk - j));
+    }
+    Flight<T, DP, KT, kWaves>::load(k0 + j * a.ks.l, a.ks.l, there, a.D, ks[buf], wave);
+    Flight<T, DP, KT, kWaves>::load(v0 + j * a.vs.l, a.vs.l, there, a.D, vs[buf], wave);
+  };
+  auto landed = [&](auto buf) {  // what load() began is there for all waves
+    if (own != nullptr && t < KT) kd[buf][t] = (there >> t & 1) ? static_cast<int>(ids) : -1;
+    range = range_next;
+    arrived<0>();
+    __syncthreads();
+  };
+  // One tile is used while the next is on its way into the other buffer.
+  int j = next();
+  auto turn = [&](auto buf) {
+    constexpr int kBuf = decltype(buf)::value;
+    const int following = next();
+    const DocRange present = range;
+    if (following >= 0) load(following, std::integral_constant<int, 1 - kBuf>());
+    if (j < most_end) {
+      bool masked = j + KT > least_end;
+      if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
+      if (masked) run.template absorb<SC, true>(a, at, qf, ks[kBuf], vs[kBuf], kd[kBuf], q, j);
+      else run.template absorb<SC, false>(a, at, qf, ks[kBuf], vs[kBuf], kd[kBuf], q, j);
+    }
+    landed(std::integral_constant<int, 1 - kBuf>());
+    j = following;
+  };
+  if (j >= 0) {
+    load(j, std::integral_constant<int, 0>());
+    landed(std::integral_constant<int, 0>());
+  }
+  while (j >= 0) {
+    turn(std::integral_constant<int, 0>());
+    if (j >= 0) turn(std::integral_constant<int, 1>());
+  }
+
+  const float total = run.l + other_half(run.l);
+  const bool none = run.top == -INFINITY && !(total != total);
+  uint32_t again = 0;
+  if (repairs<T>(a)) again = bad_columns(ok && (!finite_column(run.o) || !(fabsf(total) <= FLT_MAX)));
+  if (ok && !(again >> (lane % 32) & 1)) {
+    const float by = none ? 0.f : 1.f / total;
+    const int64_t to = ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D;
+    store_column<T, DP>(static_cast<T*>(a.o) + to, run.o, a.D, by);
+    if (a.o_rest != nullptr) store_rest<T, DP>(static_cast<T*>(a.o_rest) + to, run.o, a.D, by);
+    if (lane < 32) a.lse[bh * a.Lq + i] = none ? INFINITY : run.top + log2f(total);
+  }
+  for (; again != 0; again &= again - 1) forward_row<T>(a, b, i0 + 32 * wave + __builtin_ctz(again), h);
+}
+
+// One row's joined sums (two of the width a lane), by one wave: the quotient, or
+// the row again where it is not finite.
+template <typename T>
+DEVINL void finish_row(const AttnArgs& a, int b, int i, int h, float o0, float o1, float top, float total) {
+  const int lane = threadIdx.x % WAVE;
+  const bool none = top == -INFINITY && !(total != total);
+  if (repairs<T>(a) && __any(!(fabsf(o0) <= FLT_MAX && fabsf(o1) <= FLT_MAX && fabsf(total) <= FLT_MAX))) {
+    forward_row<T>(a, b, i, h);
+    return;
+  }
+  const float by = none ? 0.f : 1.f / total;
+  T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D;
+  o0 *= by, o1 *= by;
+  if (lane < a.D) out[lane] = from_f<T>(o0);
+  if (lane + 64 < a.D) out[lane + 64] = from_f<T>(o1);
+  if (a.o_rest != nullptr) {
+    T* rest = static_cast<T*>(a.o_rest) + ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D;
+    if (lane < a.D) rest[lane] = from_f<T>(o0 - to_f(from_f<T>(o0)));
+    if (lane + 64 < a.D) rest[lane + 64] = from_f<T>(o1 - to_f(from_f<T>(o1)));
+  }
+  if (lane == 0) a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + i] = none ? INFINITY : top + log2f(total);
+}
+
+// Few queries: a workgroup takes 32 rows (queries of all heads that share a key
+// head) and a stretch of keys, its waves every fourth 32 keys of it, each with
+// shared memory of its own, so that nothing waits but for its own loads: while one
+// tile is used the next is on its way in registers.  The waves join at the end;
+// where keys are split over workgroups too, `part` [splits, rows, DP] and `stats`
+// (maximum, sum) go to the joining kernel.
+template <typename T, int DP, Score SC>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_split_kernel(
+    AttnArgs a, const DocRange* ranges, int row_tiles, int splits, int keys_per_split, float* __restrict__ part, float2* __restrict__ stats) {
+  constexpr int KT = 32, kPad = DP + 1;
+  constexpr int kTileBytes = 2 * kWaves * KT * DP * sizeof(T), kJoinBytes = kWaves * 32 * kPad * 4;
+  __shared__ __attribute__((aligned(16))) char shared[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
+  __shared__ __attribute__((aligned(16))) int kd[kWaves][KT];
+  __shared__ float tops[kWaves][32], totals[kWaves][32];
+  const int lane = threadIdx.x % WAVE;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  T* ks = reinterpret_cast<T*>(shared) + wave * 2 * KT * DP;
+  T* vs = ks + KT * DP;
+
+  int64_t linear = blockIdx.x;  // key heads, whose rows are neighbours in memory, change fastest
+  const int kv = linear % a.Hk;
+  linear /= a.Hk;
+  const int row0 = static_cast<int>(linear % row_tiles) * 32;
+  linear /= row_tiles;
+  const int split = linear % splits, b = linear / splits;
+  const int group = a.H / a.Hk, rows = group * a.Lq;
+  const int row = row0 + lane % 32;
+  const bool ok = row < rows;
+  const int h = kv * group + (ok ? row / a.Lq : 0), i = ok ? row % a.Lq : 0;
+  const Query q = query_of(a, b, i, h, ok);
+  Frag<T> qf[DP / 16];
+  load_operands<T, DP>(q_row<T>(a, b, i, h), ok, a.D, qf);
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int x = 0; x < DP / 16; ++x) qf[x].v = -qf[x].v;
+  }
+  const int least_end = wave_min(ok ? q.end : INT_MAX), most_end = wave_max(q.end);
+  const int doc_lo = wave_min(ok ? q.doc : INT_MAX), doc_hi = wave_max(ok ? q.doc : INT_MIN);
+  const int k_tiles = (a.Lk + kDocTile - 1) / kDocTile;
+  const DocRange* own = ranges != nullptr ? ranges + static_cast<int64_t>(b) * k_tiles : nullptr;
+  const int* d0 = a.k_doc != nullptr ? a.k_doc + static_cast<int64_t>(b) * a.Lk : nullptr;
+  const T* k0 = k_row<T>(a, b, 0, kv);
+  const T* v0 = v_row<T>(a, b, 0, kv);
+  const int stop = min(most_end, (split + 1) * keys_per_split);
+
+  const Reader<T, DP> at;
+  Online<T, DP, 1> run;
+  run.clear();
+  uint32_t ids = 0;
+  DocRange range{0, 0, 0}, range_next{0, 0, 0};
+  uint64_t there = 0;
+  auto seek = [&](int j) {  // this wave's next tile of keys from j on
+    if (own != nullptr)
+      while (j < stop) {
+        range_next = own[j / kDocTile];
+        if (range_next.lo <= doc_hi && range_next.hi >= doc_lo) break;
+        j += KT * kWaves;
+      }
+    return j;
+  };
+  using Way = Flight<T, DP, KT, 1>;
+  auto load_k = [&](int j) {
+    there = first_rows(a.Lk - j);
+    if (own != nullptr) {
+      there = range_next.there >> (j % kDocTile);
+      ids = staged_word(d0 + j, lane, min(KT, a.Lk - j));
+    }
+    Way::load(k0 + j * a.ks.l, a.ks.l, there, a.D, ks, 0);
+  };
+  auto load_v = [&](int j) { Way::load(v0 + j * a.vs.l, a.vs.l, there, a.D, vs, 0); };
+  // K of the next tile is asked for as soon as the scores have read this one's, V as
+  // soon as the outputs have, so that half to all of a tile is always on its way.
+  int j = seek(split * keys_per_split + wave * KT);
+  if (j < stop) {
+    load_k(j);
+    load_v(j);
+  }
+  while (j < stop) {
+    if (own != nullptr && lane < KT) kd[wave][lane] = (there >> lane & 1) ? static_cast<int>(ids) : -1;
+    range = range_next;
+    const int following = seek(j + KT * kWaves);
+    Frag<T> p[1][2];
+    f32x16 s[1];
+    arrived<Way::kLoads>();  // K; V may still come
+    run.scores(at, qf, ks, s);
+    read_out();
+    if (following < stop) load_k(following);
+    bool masked = j + KT > least_end;
+    if (own != nullptr) masked = masked || !(range.one() && doc_lo == doc_hi && range.lo == doc_lo);
+    if (masked) run.template weights<SC, true>(a, s, p, kd[wave], q, j);
+    else run.template weights<SC, false>(a, s, p, kd[wave], q, j);
+    if (following < stop) arrived<Way::kLoads>();
+    else arrived<0>();
+    run.outputs(at, vs, p);
+    read_out();
+    if (following < stop) load_v(following);
+    j = following;
+  }
+
+  const float total = run.l + other_half(run.l);
+  if (lane < 32) tops[wave][lane] = run.top, totals[wave][lane] = total;
+  __syncthreads();  // all tiles are used: their memory takes the sums
+  float* join = reinterpret_cast<float*>(shared);
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      join[(wave * 32 + lane % 32) * kPad + 32 * x + result_row(r, lane / 32)] = run.o[x][r];
+  __syncthreads();
+  for (int c = wave; c < 32 && row0 + c < rows; c += kWaves) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w][c]);
+    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float keep = tops[w][c] == -INFINITY && top != -INFINITY ? 0.f : tops[w][c] == top ? 1.f : __builtin_amdgcn_exp2f(tops[w][c] - top);
+      sum += keep * totals[w][c];
+      o0 += keep * join[(w * 32 + c) * kPad + lane % DP];
+      if (DP > 64) o1 += keep * join[(w * 32 + c) * kPad + 64 + lane];
+    }
+    const int which = row0 + c;
+    if (splits == 1) {
+      finish_row<T>(a, b, which % a.Lq, kv * group + which / a.Lq, o0, o1, top, sum);
+    } else {
+      const int64_t to = ((static_cast<int64_t>(split) * a.B + b) * a.Hk + kv) * rows + which;
+      part[to * DP + lane] = o0;
+      if (DP > 64) part[to * DP + 64 + lane] = o1;
+      if (lane == 0) stats[to] = make_float2(top, sum);
+    }
+  }
+}
+
+// Joins the splits of a row: a wave a row, at most 64 splits.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void join_splits_kernel(AttnArgs a, int splits, int64_t count, const float* __restrict__ part,
+                                                               const float2* __restrict__ stats) {
+  const int lane = threadIdx.x % WAVE;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / WAVE;
+  if (at >= count) return;
+  const float2 own = lane < splits ? stats[lane * count + at] : make_float2(-INFINITY, 0.f);
+  float top = own.x;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, WAVE));
+  const float keep = own.x == -INFINITY && top != -INFINITY ? 0.f : own.x == top ? 1.f : __builtin_amdgcn_exp2f(own.x - top);
+  const float sum = wave_reduce_sum(keep * own.y);
+  float o0 = 0.f, o1 = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float k = lane_of(keep, s);
+    o0 += k * part[(s * count + at) * DP + lane];
+    if (DP > 64) o1 += k * part[(s * count + at) * DP + 64 + lane];
+  }
+  const int rows = a.H / a.Hk * a.Lq, row = at % rows;
+  const int64_t bc = at / rows;
+  finish_row<T>(a, bc / a.Hk, row % a.Lq, bc % a.Hk * (a.H / a.Hk) + row / a.Lq, o0, o1, top, sum);
+}
+
+// --- backward ---------------------------------------------------------------
+
+// fp16 has 2^-14 for its least normal number, and over long rows weights and score
+// gradients lie under it.  Weights are taken times 2^10 in the products over
+// queries; score gradients times a power of two that brings the largest |dO|
+// (found with delta) to 1/4 .. 1/2, so that they overflow only where a sum over the
+// width is over 2^17 times that, and then the row is done again.
+template <typename T>
+DEVINL float grad_scale(const AttnArgs& a) {
+  if (!std::is_same<T, fp16_t>::value) return 1.f;
+  const float top = __uint_as_float(*a.grad_top);
+  return top > 0.f ? exp2f(-static_cast<float>(ilogbf(top)) - 2.f) : 1.f;
+}
+
+// dQ of 32 queries a wave: lanes are queries, K and V pass by in tiles.
+//   P^T = 2^(S^T - lse), dS^T = P^T (V dO^T - delta) bend, dQ^T += K^T dS^T
+template <typename T, int DP, Score SC>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
+  constexpr int KT = sizeof(T) == 2 ? 64 : 32;
+  __shared__ __attribute__((aligned(16))) T ks[2][KT * DP];
+  __shared__ __attribute__((aligned(16))) T vs[2][KT * DP];
+  __shared__ __attribute__((aligned(16))) int kd[2][KT];
+  const int t = threadIdx.x, lane = t % WAVE;
+  const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
+  const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
+  const int64_t bh = linear / q_tiles;
+  const int i0 = (q_tiles - 1 - static_cast<int>(linear % q_tiles)) * kQueries;
+  const int b = bh / a.H, h = bh % a.H, kv = h / (a.H / a.Hk);
+  const int i = i0 + 32 * wave + lane % 32;
+  const bool ok = i < a.Lq;
+  const Query q = query_of(a, b, i, h, ok);
+  Frag<T> qf[DP / 16], gf[DP / 16];
+  load_operands<T, DP>(q_row<T>(a, b, ok ? i : 0, h), ok, a.D, qf);
+  load_operands<T, DP>(g_row<T>(a, b, ok ? i : 0, h), ok, a.D, gf);
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int x = 0; x < DP / 16; ++x) qf[x].v = -qf[x].v;
+  }
+  // dS of fp16 is scaled into its range (see grad_scale), through the exponent
+  const float lift = grad_scale<T>(a);
+  const float lse = ok ? a.lse[bh * a.Lq + i] - log2f(lift) : INFINITY, delta = ok ? a.delta[bh * a.Lq + i] : 0.f;
+  // rows that are not there decide nothing, and nothing of them is kept
+  const int least_end = wave_min(ok ? q.end : INT_MAX), most_end = wave_max(q.end);
+  const int doc_lo = wave_min(ok ? q.doc : INT_MAX), doc_hi = wave_max(ok ? q.doc : INT_MIN);
+  int lo = 0, hi = 0;
+  if (ranges != nullptr) {
+    lo = INT_MAX, hi = -1;
+#pragma unroll
+    for (int x = 0; x < kQueries; x += WAVE)
+      if (i0 + x + lane < a.Lq) {
+        const int id = a.q_doc[static_cast<int64_t>(b) * a.Lq + i0 + x + lane];
+        if (id >= 0) lo = min(lo, id);
+        hi = max(hi, id);
+      }
+    lo = wave_min(lo), hi = wave_max(hi);
+  }
+  const int j_end = a.causal ? max(0, min(a.Lk, causal_end(a, b, min(i0 + kQueries, a.Lq) - 1))) : a.Lk;
+  const int k_tiles = (a.Lk + kDocTile - 1) / kDocTile;
+  const DocRange* own = ranges != nullptr ? ranges + static_cast<int64_t>(b) * k_tiles : nullptr;
+  TileWalk walk(own, lo, hi, 0, (j_end + kDocTile - 1) / kDocTile);
+  int rest = -1;
+  auto next = [&]() {
+    if (KT < kDocTile && rest >= 0) {
+      const int j = rest;
+      rest = -1;
+      return j;
+    }
+    const int n = walk.next();
+    if (n < 0) return -1;
+    if (KT < kDocTile && n * kDocTile + KT < j_end) rest = n * kDocTile + KT;
+    return n * kDocTile;
+  };
+  const T* k0 = k_row<T>(a, b, 0, kv);
+  const T* v0 = v_row<T>(a, b, 0, kv);
+  const int* d0 = a.k_doc != nullptr ? a.k_doc + static_cast<int64_t>(b) * a.Lk : nullptr;
+
+  f32x16 dq[DP / 32];
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x) dq[x] = zeros16();
+  const Reader<T, DP> reader;
+  auto step = [&](auto masked, int j, auto buf) {
+    const Reader<T, DP> at = reader.fresh();
+#pragma unroll
+    for (int n = 0; n < KT / 32; ++n) {
+      f32x16 s = zeros16(), dp = zeros16(), bend;
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x) {
+        product(at.rows(ks[buf], 32 * n, x), qf[x], s);
+        product(at.rows(vs[buf], 32 * n, x), gf[x], dp);
+      }
+      paced<T, DP / 8, 1, 4>();
+      const float c = transform<T, SC, true>(a, s, &bend, j + 32 * n, q.at, q.slope2);
+      uint32_t seen = 0xFFFF;
+      if (masked) seen = seen_keys(a, q, kd[buf], j + 32 * n, 32 * n);
+      Frag<T> ds[2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+        if (SC == kCapped || (SC == kBiased && a.softcap > 0.f)) x *= bend[r];
+        ds[r / 8].set(r % 8, !masked || (seen >> r & 1) ? x : 0.f);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) product(at.columns(ks[buf], 32 * n + 16 * u, x), ds[u], dq[x]);
+      paced<T, DP / 16, 2, 4>();
+    }
+  };
+  uint32_t ids = 0;
+  DocRange range{0, 0, 0}, range_next{0, 0, 0};
+  uint64_t there = 0;
+  auto load = [&](int j, auto buf) {
+    there = first_rows(a.Lk - j);
+    if (own != nullptr) {
+      range_next = own[j / kDocTile];
+      there = range_next.there >> (j % kDocTile);
+      ids = staged_word(d0 + j, t, min(KT, a.Lk - j));
+    }
+    Flight<T, DP, KT, kWaves>::load(k0 + j * a.ks.l, a.ks.l, there, a.D, ks[buf], wave);
+    Flight<T, DP, KT, kWaves>::load(v0 + j * a.vs.l, a.vs.l, there, a.D, vs[buf], wave);
+  };
+  auto landed = [&](auto buf) {  // what load() began is there for all waves
+    if (own != nullptr && t < KT) kd[buf][t] = (there >> t & 1) ? static_cast<int>(ids) : -1;
+    range = range_next;
+    arrived<0>();
+    __syncthreads();
+  };
+  // One tile is used while the next is on its way into the other buffer.
+  int j = next();
+  auto turn = [&](auto buf) {
+    constexpr int kBuf = decltype(buf)::value;
+    const int following = next();
+    const DocRange present = range;
+    if (following >= 0) load(following, std::integral_constant<int, 1 - kBuf>());
+    if (j < most_end) {
+      bool masked = j + KT > least_end;
+      if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
+      if (masked) step(std::true_type(), j, buf);
+      else step(std::false_type(), j, buf);
+    }
+    landed(std::integral_constant<int, 1 - kBuf>());
+    j = following;
+  };
+  if (j >= 0) {
+    load(j, std::integral_constant<int, 0>());
+    landed(std::integral_constant<int, 0>());
+  }
+  while (j >= 0) {
+    turn(std::integral_constant<int, 0>());
+    if (j >= 0) turn(std::integral_constant<int, 1>());
+  }
+
+  uint32_t again = 0;
+  if (repairs<T>(a)) again = bad_columns(ok && !finite_column(dq));
+  if (ok && !(again >> (lane % 32) & 1))
+    store_column<T, DP>(static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D, dq, a.D, a.scale / lift);
+  for (; again != 0; again &= again - 1) dq_row<T>(a, b, i0 + 32 * wave + __builtin_ctz(again), h);
+}
+
+// dK and dV of 32 keys a wave: lanes are keys, Q and dO of all heads that share
+// them pass by in tiles.
+//   P = 2^(S - lse), dV^T += dO^T P, dS = P (dO V^T - delta) bend, dK^T += Q^T dS
+template <typename T, int DP, Score SC>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void dkv_tiles_kernel(AttnArgs a, const DocRange* ranges, int k_blocks, int splits, float* __restrict__ part) {
+  constexpr int QT = sizeof(T) == 2 ? 64 : 32, kKeys = 32 * kWaves;
+  __shared__ __attribute__((aligned(16))) T qs[2][QT * DP];
+  __shared__ __attribute__((aligned(16))) T gs[2][QT * DP];
+  __shared__ __attribute__((aligned(16))) float stats[2][2][QT];  // lse, delta
+  __shared__ __attribute__((aligned(16))) int qd[2][QT];
+  const int t = threadIdx.x, lane = t % WAVE, half = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
+  const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
+  const int split = linear % splits;
+  const int64_t bc = linear / splits / k_blocks;
+  const int j0 = static_cast<int>(linear / splits % k_blocks) * kKeys;
+  const int b = bc / a.Hk, kv = bc % a.Hk, group = a.H / a.Hk, off = a.Lk - a.Lq;
+  const int j = j0 + 32 * wave + lane % 32;
+  const int doc = j < a.Lk && a.k_doc != nullptr ? a.k_doc[static_cast<int64_t>(b) * a.Lk + j] : 0;
+  const bool in = j < a.Lk, ok = in && doc >= 0;
+  Frag<T> kf[DP / 16], vf[DP / 16];
+  load_operands<T, DP>(k_row<T>(a, b, ok ? j : 0, kv), ok, a.D, kf);
+  load_operands<T, DP>(v_row<T>(a, b, ok ? j : 0, kv), ok, a.D, vf);
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int x = 0; x < DP / 16; ++x) kf[x].v = -kf[x].v;
+  }
+  // the first query that sees a key
+  const int prefix = a.prefix != nullptr ? a.prefix[b] : 0;
+  const int begin = !ok ? INT_MAX : !a.causal || j < prefix ? 0 : max(0, j - off);
+  const int least_begin = wave_min(begin), most_begin = wave_max(begin);
+  const int doc_lo = wave_min(doc), doc_hi = wave_max(doc);
+  int lo = 0, hi = 0;
+  if (ranges != nullptr) {
+    lo = INT_MAX, hi = -1;
+#pragma unroll
+    for (int x = 0; x < kKeys; x += WAVE)
+      if (j0 + x + lane < a.Lk) {
+        const int id = a.k_doc[static_cast<int64_t>(b) * a.Lk + j0 + x + lane];
+        if (id >= 0) lo = min(lo, id);
+        hi = max(hi, id);
+      }
+    lo = wave_min(lo), hi = wave_max(hi);
+  }
+  const int i_begin = !a.causal || j0 < prefix ? 0 : max(0, j0 - off);
+  const int q_tiles = (a.Lq + kDocTile - 1) / kDocTile;
+  const DocRange* own = ranges != nullptr ? ranges + static_cast<int64_t>(b) * q_tiles : nullptr;
+  // the workgroup's part of the (head, tile) pairs: even stretches of them
+  const int first_tile = min(i_begin / kDocTile, q_tiles), per_head = q_tiles - first_tile;
+  const int64_t units = static_cast<int64_t>(group) * per_head;
+  const int64_t unit_begin = units * split / splits, unit_end = units * (split + 1) / splits;
+  int64_t unit = unit_begin;  // where the walk of the present head began
+  int head = kv * group, rest = -1;
+  TileWalk walk(own, lo, hi, 0, 0);
+  auto enter = [&]() {  // the head that holds `unit`
+    const int g = static_cast<int>(unit / per_head);
+    const int64_t base = static_cast<int64_t>(g) * per_head;
+    head = kv * group + g;
+    walk = TileWalk(own, lo, hi, first_tile + static_cast<int>(unit - base),
+                    first_tile + static_cast<int>(min(static_cast<int64_t>(per_head), unit_end - base)));
+    unit = base + per_head;
+  };
+  auto next = [&](int& at_head) {
+    if (QT < kDocTile && rest >= 0) {
+      const int i = rest;
+      rest = -1;
+      at_head = head;
+      return i;
+    }
+    int n = walk.next();
+    while (n < 0) {
+      if (unit >= unit_end) return -1;
+      enter();
+      n = walk.next();
+    }
+    if (QT < kDocTile && n * kDocTile + QT < a.Lq) rest = n * kDocTile + QT;
+    at_head = head;
+    return n * kDocTile;
+  };
+  constexpr float kWeightLift = sizeof(T) == 2 && std::is_same<T, fp16_t>::value ? 10.f : 0.f;  // see grad_scale
+  const float lift = grad_scale<T>(a);
+  const int* d0 = a.q_doc != nullptr ? a.q_doc + static_cast<int64_t>(b) * a.Lq : nullptr;
+
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int x = 0; x < DP / 32; ++x) dk[x] = zeros16(), dv[x] = zeros16();
+  const Reader<T, DP> reader;
+  auto step = [&](auto masked, int i, float slope2, auto buf) {
+    const Reader<T, DP> at = reader.fresh();
+#pragma unroll
+    for (int n = 0; n < QT / 32; ++n) {
+      f32x16 s = zeros16(), dp = zeros16(), bend;
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x) {
+        product(at.rows(qs[buf], 32 * n, x), kf[x], s);
+        product(at.rows(gs[buf], 32 * n, x), vf[x], dp);
+      }
+      paced<T, DP / 8, 1, 4>();
+      // the distance |i + off - j| with queries in registers: as if the key stood at j - off
+      const float c = transform<T, SC, true>(a, s, &bend, i + 32 * n, j - off, slope2);
+      uint32_t seen = 0xFFFF;
+      if (masked) {
+        seen = 0;
+        const int from = begin == INT_MAX ? INT_MAX : begin - i - 32 * n - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) seen |= static_cast<uint32_t>(result_row(r, 0) >= from) << r;
+        if (own != nullptr) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int4 d = *reinterpret_cast<const int4*>(&qd[buf][32 * n + 8 * x + 4 * half]);
+            const uint32_t same = static_cast<uint32_t>(d.x == doc) | static_cast<uint32_t>(d.y == doc) << 1 |
+                                  static_cast<uint32_t>(d.z == doc) << 2 | static_cast<uint32_t>(d.w == doc) << 3;
+            seen &= same << (4 * x) | ~(15u << (4 * x));
+          }
+        }
+      }
+      Frag<T> p[2], ds[2];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float4 lse = *reinterpret_cast<const float4*>(&stats[buf][0][32 * n + 8 * x + 4 * half]);
+        const float4 del = *reinterpret_cast<const float4*>(&stats[buf][1][32 * n + 8 * x + 4 * half]);
+        const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int r = 4 * x + y;
+          const float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ls[y]));
+          float g = w * (dp[r] - de[y]);
+          if (SC == kCapped || (SC == kBiased && a.softcap > 0.f)) g *= bend[r];
+          if (std::is_same<T, fp16_t>::value) g *= lift;
+          const bool sees = !masked || (seen >> r & 1);
+          p[r / 8].set(r % 8, sees ? w : 0.f);
+          ds[r / 8].set(r % 8, sees ? g : 0.f);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 0; x < DP / 32; ++x) {
+          product(at.columns(gs[buf], 32 * n + 16 * u, x), p[u], dv[x]);
+          product(at.columns(qs[buf], 32 * n + 16 * u, x), ds[u], dk[x]);
+        }
+      paced<T, DP / 8, 2, 4>();
+    }
+  };
+  uint32_t ids = 0, stat = 0;
+  DocRange range{0, 0, 0}, range_next{0, 0, 0};
+  uint64_t there = 0;
+  auto load = [&](int i, int h, auto buf) {
+    there = first_rows(a.Lq - i);
+    const int rows = min(QT, a.Lq - i);
+    const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.Lq + i;
+    stat = staged_word((wave == 0 ? a.lse : a.delta) + row, lane, wave < 2 ? rows : 0);  // one wave brings lse, one delta
+    if (own != nullptr) {
+      range_next = own[i / kDocTile];
+      there = range_next.there >> (i % kDocTile);
+      ids = staged_word(d0 + i, t, rows);
+    }
+    Flight<T, DP, QT, kWaves>::load(q_row<T>(a, b, i, h), a.qs.l, there, a.D, qs[buf], wave);
+    Flight<T, DP, QT, kWaves>::load(g_row<T>(a, b, i, h), a.gs.l, there, a.D, gs[buf], wave);
+  };
+  auto landed = [&](auto buf) {
+    const bool here = there >> lane & 1;
+    if (wave == 0 && lane < QT) stats[buf][0][lane] = here ? __uint_as_float(stat) - kWeightLift : INFINITY;
+    if (wave == 1 && lane < QT) stats[buf][1][lane] = here ? __uint_as_float(stat) : 0.f;
+    if (own != nullptr && t < QT) qd[buf][t] = here ? static_cast<int>(ids) : -1;
+    range = range_next;
+    arrived<0>();
+    __syncthreads();
+  };
+  int h = head, h_next = head;
+  int i = next(h);
+  auto turn = [&](auto buf) {
+    constexpr int kBuf = decltype(buf)::value;
+    const int following = next(h_next);
+    const DocRange present = range;
+    if (following >= 0) load(following, h_next, std::integral_constant<int, 1 - kBuf>());
+    if (i + QT > least_begin) {
+      const float slope2 = a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
+      bool masked = i < most_begin;
+      if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
+      if (masked) step(std::true_type(), i, slope2, buf);
+      else step(std::false_type(), i, slope2, buf);
+    }
+    landed(std::integral_constant<int, 1 - kBuf>());
+    i = following;
+    h = h_next;
+  };
+  if (i >= 0) {
+    load(i, h, std::integral_constant<int, 0>());
+    landed(std::integral_constant<int, 0>());
+  }
+  while (i >= 0) {
+    turn(std::integral_constant<int, 0>());
+    if (i >= 0) turn(std::integral_constant<int, 1>());
+  }
+  const float drop = exp2f(-kWeightLift);
+  if (splits > 1) {  // joined, and looked at, by the next kernel
+    const int64_t to = ((static_cast<int64_t>(b) * a.Lk + j) * a.Hk + kv) * a.D, all = static_cast<int64_t>(a.B) * a.Lk * a.Hk * a.D;
+    if (in) {
+      store_column<float, DP>(part + 2 * split * all + to, dk, a.D, a.scale / lift * drop);
+      store_column<float, DP>(part + (2 * split + 1) * all + to, dv, a.D, drop);
+    }
+    return;
+  }
+  uint32_t again = 0;
+  if (repairs<T>(a)) again = bad_columns(in && !(finite_column(dk) && finite_column(dv)));
+  if (in && !(again >> (lane % 32) & 1)) {
+    const int64_t out = ((static_cast<int64_t>(b) * a.Lk + j) * a.Hk + kv) * a.D;
+    store_column<T, DP>(static_cast<T*>(a.dk) + out, dk, a.D, a.scale / lift * drop);
+    store_column<T, DP>(static_cast<T*>(a.dv) + out, dv, a.D, drop);
+  }
+  for (; again != 0; again &= again - 1) dkv_row<T>(a, b, j0 + 32 * wave + __builtin_ctz(again), kv);
+}
+
+// Sums the parts of dK and dV in their order: a wave a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_dkv_kernel(AttnArgs a, int splits, int64_t rows, const float* __restrict__ part) {
+  const int lane = threadIdx.x % WAVE;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / WAVE, all = rows * a.D;
+  if (row >= rows) return;
+  float dk[2] = {0.f, 0.f}, dv[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (lane + 64 * x < a.D) {
+        dk[x] += part[2 * s * all + row * a.D + lane + 64 * x];
+        dv[x] += part[(2 * s + 1) * all + row * a.D + lane + 64 * x];
+      }
+  const bool fine = fabsf(dk[0]) <= FLT_MAX && fabsf(dk[1]) <= FLT_MAX && fabsf(dv[0]) <= FLT_MAX && fabsf(dv[1]) <= FLT_MAX;
+  if (repairs<T>(a) && __any(!fine)) {
+    const int64_t bl = row / a.Hk;
+    dkv_row<T>(a, bl / a.Lk, bl % a.Lk, row % a.Hk);
+    return;
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    if (lane + 64 * x < a.D) {
+      static_cast<T*>(a.dk)[row * a.D + lane + 64 * x] = from_f<T>(dk[x]);
+      static_cast<T*>(a.dv)[row * a.D + lane + 64 * x] = from_f<T>(dv[x]);
+    }
+}
+
+// delta[b, h, i] = sum_d dout o: sixteen lanes a row.  o is taken with what its
+// rounding left: delta is subtracted from every dP of a row, so that its error does
+// not average out, and with o in 16 bits it was the largest in dQ and dK.
+// `top`: the bits of the largest finite |dout|, or null: a maximum does not depend on
+// the order it is taken in, and a workgroup brings one.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void delta_kernel(AttnArgs a, float* __restrict__ delta, unsigned* __restrict__ top, int64_t rows) {
+  __shared__ float highs[kWaves];
+  const int t = threadIdx.x % 16;
+  float high = 0.f;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + threadIdx.x / 16; row < rows;
+       row += static_cast<int64_t>(gridDim.x) * (kThreads / 16)) {
+    const int64_t bl = row / a.H;
+    const int h = row % a.H, b = bl / a.Lq, i = bl % a.Lq;
+    const T* g = g_row<T>(a, b, i, h);
+    const T* o = static_cast<const T*>(a.o) + row * a.D;
+    float s = 0.f;
+    if (t * 8 < a.D) {
+      float x[8], y[8];
+      load8(g + t * 8, x);
+      load8(o + t * 8, y);
+      if (a.o_rest != nullptr) {
+        float rest[8];
+        load8(static_cast<const T*>(a.o_rest) + row * a.D + t * 8, rest);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] += rest[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s = fmaf(x[e], y[e], s);
+        if (fabsf(x[e]) <= FLT_MAX) high = fmaxf(high, fabsf(x[e]));
+      }
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor(s, off, 16);  // sixteen lanes leave the loop together
+    if (t == 0) delta[(static_cast<int64_t>(b) * a.H + h) * a.Lq + i] = s;
+  }
+  if (top == nullptr) return;
+  high = wave_reduce_max(high);
+  if (threadIdx.x % WAVE == 0) highs[threadIdx.x / WAVE] = high;
+  __syncthreads();
+  if (threadIdx.x == 0) atomicMax(top, __float_as_uint(fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3]))));
+}
+
+int blocks_for(int64_t items, int64_t each) {
+  const int64_t n = (items + each - 1) / each;
+  TORCH_CHECK(n < (int64_t{1} << 31), "attention: too many rows");
+  return static_cast<int>(n);
+}
+
+constexpr int kComputeUnits = 256;
+
+// Calls `fn` with the padded width and what scores go through as constants.
+template <typename Fn>
+void with_variant(const AttnArgs& a, Fn fn) {
+  auto by_score = [&](auto width) {
+    if (a.slopes != nullptr || a.scale == 0.f) fn(width, std::integral_constant<Score, kBiased>());
+    else if (a.softcap > 0.f) fn(width, std::integral_constant<Score, kCapped>());
+    else fn(width, std::integral_constant<Score, kPlain>());
+  };
+  if (a.D <= 64) by_score(std::integral_constant<int, 64>());
+  else by_score(std::integral_constant<int, 128>());
+}
+
+// Tiles of queries where they fill the chip and their 128 rows are mostly there; 32
+// rows and stretches of keys where not.
+template <typename T, int DP, Score SC>
+void run_forward(const AttnArgs& a, const DocRange* ranges, const torch::TensorOptions& options, hipStream_t stream) {
+  const int64_t tiles = static_cast<int64_t>(a.B) * a.H * ((a.Lq + kQueries - 1) / kQueries);
+  if (tiles >= kComputeUnits && a.Lq >= 64) {
+    forward_tiles_kernel<T, DP, SC><<<blocks_for(tiles, 1), kThreads, 0, stream>>>(a, ranges, (a.Lq + kQueries - 1) / kQueries);
+    return;
+  }
+  const int rows = a.H / a.Hk * a.Lq, row_tiles = (rows + 31) / 32;
+  const int64_t groups = static_cast<int64_t>(a.B) * a.Hk * row_tiles, count = static_cast<int64_t>(a.B) * a.Hk * rows;
+  // some eight workgroups a CU, so that rows of uneven length even out, but 512
+  // keys for each
+  const int splits = std::max<int64_t>(1, std::min<int64_t>({64, (8 * kComputeUnits + groups - 1) / groups, a.Lk / 512}));
+  const int each = ((a.Lk + splits - 1) / splits + 127) / 128 * 128;
+  const int used = (a.Lk + each - 1) / each;
+  torch::Tensor part, stats;
+  if (used > 1) {
+    part = torch::empty({used, count, DP}, options.dtype(at::kFloat));
+    stats = torch::empty({used, count, 2}, options.dtype(at::kFloat));
+  }
+  float* p = used > 1 ? part.data_ptr<float>() : nullptr;
+  float2* st = used > 1 ? reinterpret_cast<float2*>(stats.data_ptr<float>()) : nullptr;
+  forward_split_kernel<T, DP, SC><<<blocks_for(groups * used, 1), kThreads, 0, stream>>>(a, ranges, row_tiles, used, each, p, st);
+  if (used > 1) join_splits_kernel<T, DP><<<blocks_for(count, kWaves), kThreads, 0, stream>>>(a, used, count, p, st);
+}
+
+template <typename T, int DP, Score SC>
+void run_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q_ranges, const torch::TensorOptions& options, hipStream_t stream) {
+  const int q_tiles = (a.Lq + kQueries - 1) / kQueries, k_blocks = (a.Lk + kQueries - 1) / kQueries;
+  dq_tiles_kernel<T, DP, SC><<<blocks_for(static_cast<int64_t>(a.B) * a.H * q_tiles, 1), kThreads, 0, stream>>>(a, k_ranges, q_tiles);
+  // Blocks of keys that do not fill the chip four times over are split over heads and
+  // queries, down to eight tiles of queries, for their sums to be joined: a causal
+  // mask makes their lengths uneven, and heads that share keys make them few.
+  const int64_t base = static_cast<int64_t>(a.B) * a.Hk * k_blocks;
+  const int64_t tiles = static_cast<int64_t>(a.H / a.Hk) * ((a.Lq + kDocTile - 1) / kDocTile);
+  const int splits = std::max<int64_t>(1, std::min<int64_t>(4 * kComputeUnits / base, tiles / 8));
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Lk * a.Hk;
+  torch::Tensor part;
+  if (splits > 1) part = torch::empty({splits, 2, rows, a.D}, options.dtype(at::kFloat));
+  float* p = splits > 1 ? part.data_ptr<float>() : nullptr;
+  dkv_tiles_kernel<T, DP, SC><<<blocks_for(base * splits, 1), kThreads, 0, stream>>>(a, q_ranges, k_blocks, splits, p);
+  if (splits > 1) join_dkv_kernel<T><<<blocks_for(rows, kWaves), kThreads, 0, stream>>>(a, splits, rows, p);
+}
+
+}  // namespace
+
+template <typename T>
+void attention_forward(const AttnArgs& a, const DocRange* ranges, const torch::TensorOptions& options, hipStream_t stream) {
+  with_variant(a, [&](auto width, auto score) {
+    run_forward<T, decltype(width)::value, decltype(score)::value>(a, ranges, options, stream);
+  });
+}
+
+template <typename T>
+void attention_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q_ranges, const torch::TensorOptions& options,
+                        hipStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.B) * a.H * a.Lq;
+  delta_kernel<T><<<std::min(blocks_for(rows, kThreads / 16), 8 * kComputeUnits), kThreads, 0, stream>>>(
+      a, const_cast<float*>(a.delta), const_cast<unsigned*>(a.grad_top), rows);
+  with_variant(a, [&](auto width, auto score) {
+    run_backward<T, decltype(width)::value, decltype(score)::value>(a, k_ranges, q_ranges, options, stream);
+  });
+}

@@ -53,6 +53,24 @@ DEVINL void product(const Frag<float>& a, const Frag<float>& b, f32x16& c) {
   for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
 }
 
+// The order of a block of N products and the reads of shared memory that bring one
+// operand of each (READS instructions): AHEAD operands first, then a product for
+// every further one, so that a read's latency passes under products, and no more
+// registers are taken than that.  Nothing moves across its ends.
+template <typename T, int N, int READS, int AHEAD>
+DEVINL void paced() {
+  if constexpr (sizeof(T) == 2) {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 DEVINL f32x16 zeros16() {
   f32x16 z;
 #pragma unroll
@@ -72,79 +90,115 @@ struct Tile {
   }
   static DEVINL int chunk_at(int row, int c) { return row * kChunks + (c ^ swizzle(row)); }
 
-  // Row row0 + lane % 32, k = 16 step + 8 half ...: an operand as it lies.
-  static DEVINL Frag<T> rows(const T* tile, int row0, int step) {
-    const int lane = threadIdx.x % WAVE, row = row0 + lane % 32, half = lane / 32;
-    Frag<T> f;
-    const u32x4* p = reinterpret_cast<const u32x4*>(tile);
-    u32x4* out = reinterpret_cast<u32x4*>(&f.v);
-    if constexpr (sizeof(T) == 2) {
-      out[0] = p[chunk_at(row, 2 * step + half)];
+};
+
+// A wave's way of reading operands from a tile.  A lane's places differ from its
+// first by constants, under XOR (the swizzle is linear in the bits of the row) and in
+// the offset: two registers hold all of them, and `fresh` keeps the compiler from
+// holding every one over the loop instead.
+template <typename T, int DP>
+struct Reader {
+  using Tl = Tile<T, DP>;
+  static constexpr bool kWide = sizeof(T) == 4;
+  int row_at;  // elements: row lane % 32, its eight k of step 0
+  int col_at;  // elements: a lane's place for columns, x = 0, its first row
+
+  DEVINL Reader() {
+    const int lane = threadIdx.x % WAVE, half = lane / 32;
+    row_at = Tl::chunk_at(lane % 32, (kWide ? 2 : 1) * half) * Tl::kPer;
+    if constexpr (kWide) {
+      col_at = Tl::chunk_at(4 * half, lane % 32 / 4) * 4 + lane % 4;
     } else {
-      out[0] = p[chunk_at(row, 4 * step + 2 * half)];
-      out[1] = p[chunk_at(row, 4 * step + 2 * half + 1)];
+      const int j = lane % 16, col = lane / 16 % 2 * 16 + j % 4 * 4;
+      col_at = Tl::chunk_at(4 * half + j / 4, col / 8) * 8 + col % 8;
     }
+  }
+
+  DEVINL Reader fresh() const {
+    Reader r = *this;
+    asm volatile("" : "+v"(r.row_at), "+v"(r.col_at));
+    return r;
+  }
+
+  // Row row0 + lane % 32 (row0 a multiple of 16), k = 16 step + 8 half ...: an
+  // operand as it lies.
+  DEVINL Frag<T> rows(const T* tile, int row0, int step) const {
+    Frag<T> f;
+    u32x4* out = reinterpret_cast<u32x4*>(&f.v);
+    out[0] = *reinterpret_cast<const u32x4*>(tile + row0 * DP + (row_at ^ 16 * step));
+    if constexpr (kWide) out[1] = *reinterpret_cast<const u32x4*>(tile + row0 * DP + (row_at ^ 16 * step ^ 4));
     return f;
   }
 
-  // Column d0 + lane % 32 of rows row0 .. row0 + 15, in the order of results:
-  // an operand transposed.
-  static DEVINL Frag<T> columns(const T* tile, int row0, int d0) {
-    const int lane = threadIdx.x % WAVE, half = lane / 32;
+  // Column 32 x + lane % 32 of rows row0 .. row0 + 15 (row0 a multiple of 16), in
+  // the order of results: an operand transposed.
+  DEVINL Frag<T> columns(const T* tile, int row0, int x) const {
     Frag<T> f;
-    if constexpr (sizeof(T) == 2) {
-      const int j = lane % 16;
-      const int col = d0 + (lane / 16) % 2 * 16 + j % 4 * 4;
-      s16x4* out = reinterpret_cast<s16x4*>(&f.v);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int row = row0 + 8 * x + 4 * half + j / 4;
-        const T* p = tile + chunk_at(row, col / 8) * 8 + col % 8;
-        out[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(const_cast<T*>(p)));
-      }
-    } else {
-      const int col = d0 + lane % 32;
+    if constexpr (kWide) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int row = row0 + 8 * (i / 4) + 4 * half + i % 4;
-        f.v[i] = tile[chunk_at(row, col / 4) * 4 + col % 4];
+        const int row = 8 * (i / 4) + i % 4;
+        f.v[i] = tile[(row0 + row) * DP + (col_at ^ 32 * x ^ Tl::swizzle(row) * 4)];
       }
+    } else {
+      s16x4* out = reinterpret_cast<s16x4*>(&f.v);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        out[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(const_cast<T*>(tile + (row0 + 8 * i) * DP + (col_at ^ 32 * x ^ Tl::swizzle(8 * i) * 8))));
     }
     return f;
   }
 };
 
-// Global rows on their way to shared memory, in registers: NT threads, ROWS rows.
-// Rows from `count` on, chunks behind the width and rows whose id is negative
-// come as zeros (an offset beyond the buffer's end reads as zero).
-template <typename T, int DP, int ROWS, int NT>
-struct Staged {
+// Global rows straight to a tile in shared memory, 16 bytes a lane, by WAVES waves.
+// A load writes its lanes' chunks one behind another, so each lane asks for the chunk
+// that belongs at its place: within a tile rows n steps apart differ by a constant in
+// the swizzle.  Rows without their bit in `there` and chunks behind the width come
+// as zeros (an offset beyond the buffer's end reads as zero).  Nothing waits here:
+// `arrived` does, and the compiler knows of no dependence.
+template <typename T, int DP, int ROWS, int WAVES>
+struct Flight {
   using Tl = Tile<T, DP>;
-  static constexpr int kEach = ROWS * Tl::kChunks / NT;
-  static_assert(ROWS * Tl::kChunks % NT == 0, "threads share the chunks evenly");
-  u32x4 r[kEach];
+  static constexpr int kStep = WAVES * WAVE / Tl::kChunks;  // rows of one load of all waves
+  static constexpr int kLoads = ROWS / kStep;
+  static_assert(ROWS % kStep == 0 && (kStep & (kStep - 1)) == 0, "waves share the rows evenly");
 
-  DEVINL void load(const T* base, int64_t row_stride, int count, int D, const int* doc, int t) {
+  static DEVINL void load(const T* base, int64_t row_stride, uint64_t there, int D, T* tile, int wave) {
     auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7FFFFFFF, 0x00020000);
+    const int stride = static_cast<int>(row_stride) * static_cast<int>(sizeof(T));
+    const int place = wave * WAVE + threadIdx.x % WAVE;
+    const int row = place / Tl::kChunks, c = place % Tl::kChunks ^ Tl::swizzle(row);
+    const int at = row * stride;
+    // full tiles of full rows need no look at every row
+    const bool full = D == DP && (ROWS == 32 ? static_cast<uint32_t>(there) == ~0u : there == ~uint64_t{0});
 #pragma unroll
-    for (int n = 0; n < kEach; ++n) {
-      const int i = t + n * NT, row = i / Tl::kChunks, c = i % Tl::kChunks;
-      bool ok = row < count && c * Tl::kPer < D;
-      if (doc != nullptr && ok) ok = doc[row] >= 0;
-      const int at = static_cast<int>(row * row_stride + c * Tl::kPer) * static_cast<int>(sizeof(T));
-      r[n] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, ok ? at : -1, 0, 0);
-    }
-  }
-
-  DEVINL void store(T* tile, int t) const {
-#pragma unroll
-    for (int n = 0; n < kEach; ++n) {
-      const int i = t + n * NT, row = i / Tl::kChunks, c = i % Tl::kChunks;
-      reinterpret_cast<u32x4*>(tile)[Tl::chunk_at(row, c)] = r[n];
+    for (int n = 0; n < kLoads; ++n) {
+      const int chunk = c ^ Tl::swizzle(n * kStep);
+      int from = at + chunk * 16;
+      if (!full) from = (there >> (row + n * kStep) & 1) && chunk * Tl::kPer < D ? from : -1;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void*)(tile + (n * WAVES + wave) * WAVE * Tl::kPer), 16, from, n * kStep * stride, 0, 0);
     }
   }
 };
+
+// All but the last `N` loads of this wave are in shared memory.
+template <int N>
+DEVINL void arrived() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// All reads of shared memory of this wave are in registers.
+DEVINL void read_out() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// One word a thread, the first `n` of them, on the same way.
+DEVINL uint32_t staged_word(const void* base, int t, int n) {
+  auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+  return __builtin_amdgcn_raw_buffer_load_b32(rsrc, t < n ? 4 * t : -1, 0, 0);
+}
+
+// The first `n` of 64 rows, as bits.
+DEVINL uint64_t first_rows(int n) { return n >= 64 ? ~uint64_t{0} : n <= 0 ? 0 : (uint64_t{1} << n) - 1; }
 
 // Row `row` (per lane) of q or dO straight into operands: k = 16 step + 8 half ...
 template <typename T, int DP>
@@ -179,9 +233,13 @@ DEVINL int64_t xcd_order(int64_t i, int64_t n) {
   return x * each + min(x, more) + i / 8;
 }
 
-// The ids of 64 rows (of one batch row): {least, largest, 1 if all 64 are one
-// id >= 0}; negative ids do not count, and without any the range is empty.
-struct DocRange { int lo, hi, one, pad; };
+// The ids of 64 rows (of one batch row): the least and largest that are not
+// negative (an empty range without any), and which rows have one.
+struct DocRange {
+  int lo, hi;
+  uint64_t there;
+  DEVINL bool one() const { return lo == hi && there == ~uint64_t{0}; }
+};
 constexpr int kDocTile = 64;
 
 // Which tiles of 64 rows an interval of ids may meet: 64 of them at a time.

@@ -85,9 +85,9 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
 std::vector<torch::Tensor> attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double softcap,
                                          c10::optional<torch::Tensor> slopes, bool causal,
                                          c10::optional<torch::Tensor> prefix, c10::optional<torch::Tensor> q_doc,
-                                         c10::optional<torch::Tensor> k_doc);
+                                         c10::optional<torch::Tensor> k_doc, bool keep_rest);
 std::vector<torch::Tensor> attention_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
-                                         torch::Tensor o, torch::Tensor lse, double scale, double softcap,
+                                         torch::Tensor o, torch::Tensor lse, torch::Tensor rest, double scale, double softcap,
                                          c10::optional<torch::Tensor> slopes, bool causal,
                                          c10::optional<torch::Tensor> prefix, c10::optional<torch::Tensor> q_doc,
                                          c10::optional<torch::Tensor> k_doc);

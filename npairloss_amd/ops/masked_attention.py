@@ -117,7 +117,7 @@ def _ready(x, width):
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, scale, softcap, slopes, causal, prefix, q_doc, k_doc):
+    def forward(ctx, q, k, v, scale, softcap, slopes, causal, prefix, q_doc, k_doc, train):
         how = (scale, softcap, slopes, causal, prefix, q_doc, k_doc)
         ctx.how, ctx.width = (scale, softcap, causal), q.shape[-1]
         ctx.empty = q.numel() == 0 or k.numel() == 0
@@ -127,25 +127,25 @@ class _AttentionFn(torch.autograd.Function):
         if q.is_cuda:
             width = -(-ctx.width // 8) * 8
             q, k, v = (_ready(x, width) for x in (q, k, v))
-            o, lse = _backend.ext().attention_fwd(q, k, v, *how)
+            o, lse, rest = _backend.ext().attention_fwd(q, k, v, *how, train)
         else:
-            o, lse = _forward_torch(q, k, v, *how)
-        ctx.save_for_backward(q, k, v, o, lse, slopes, prefix, q_doc, k_doc)
+            (o, lse), rest = _forward_torch(q, k, v, *how), None
+        ctx.save_for_backward(q, k, v, o, lse, rest, slopes, prefix, q_doc, k_doc)
         return o[..., :ctx.width]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         if ctx.empty:
-            return tuple(torch.zeros_like(x) for x in ctx.saved_tensors) + (None,) * 7
-        q, k, v, o, lse, slopes, prefix, q_doc, k_doc = ctx.saved_tensors
+            return tuple(torch.zeros_like(x) for x in ctx.saved_tensors) + (None,) * 8
+        q, k, v, o, lse, rest, slopes, prefix, q_doc, k_doc = ctx.saved_tensors
         scale, softcap, causal = ctx.how
         how = (scale, softcap, slopes, causal, prefix, q_doc, k_doc)
         if q.is_cuda:
-            grads = _backend.ext().attention_bwd(_ready(g, q.shape[-1]), q, k, v, o, lse, *how)
+            grads = _backend.ext().attention_bwd(_ready(g, q.shape[-1]), q, k, v, o, lse, rest, *how)
         else:
             grads = _backward_torch(g, q, k, v, o, lse, *how)
-        return tuple(x[..., :ctx.width] for x in grads) + (None,) * 7
+        return tuple(x[..., :ctx.width] for x in grads) + (None,) * 8
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, softcap: float = 0.0,
@@ -200,4 +200,5 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
             raise ValueError(f"attention: tensors on {q.device} and {x.device}")
     slopes, prefix, documents, key_documents = (x if x is None else x.detach().contiguous()
                                                 for x in (slopes, prefix, documents, key_documents))
-    return _AttentionFn.apply(q, k, v, scale, float(softcap), slopes, bool(causal), prefix, documents, key_documents)
+    train = torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v))
+    return _AttentionFn.apply(q, k, v, scale, float(softcap), slopes, bool(causal), prefix, documents, key_documents, train)

@@ -11,8 +11,8 @@ Usage:  python setup.py build_ext --inplace   (or just: python setup.py)
 """
 
 import concurrent.futures
-import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -38,6 +38,9 @@ SOURCES = [
     "rotary.hip",
     "adamw.hip",
     "attention.hip",
+    "attention_f32.hip",
+    "attention_bf16.hip",
+    "attention_fp16.hip",
 ]
 
 
@@ -78,12 +81,23 @@ def compile_flags(tdir):
     ]
 
 
+def headers(path, seen=None):
+    """The headers of csrc/ that a source includes, directly or not."""
+    seen = set() if seen is None else seen
+    with open(path) as f:
+        for name in re.findall(r'^#include "(.+?)"', f.read(), re.M):
+            h = os.path.join(CSRC, name)
+            if os.path.exists(h) and h not in seen:
+                seen.add(h)
+                headers(h, seen)
+    return seen
+
+
 def needs_build(src, obj):
     if not os.path.exists(obj):
         return True
-    dep = [src, os.path.abspath(__file__)] + glob.glob(os.path.join(CSRC, "*.h"))
     omt = os.path.getmtime(obj)
-    return any(os.path.getmtime(d) > omt for d in dep if os.path.exists(d))
+    return any(os.path.getmtime(d) > omt for d in [src, os.path.abspath(__file__), *headers(src)])
 
 
 def build(verbose=True, force=False):
