@@ -33,8 +33,8 @@ struct AttnArgs {
   const int* k_doc;      // [B, Lk] or null
   // backward
   const void* dout; RowStrides gs;
-  const float* delta;    // [B, H, Lq]: sum_d dout o
-  const unsigned* grad_top;  // bits of the largest |dout| (fp16) or null
+  float* delta;          // [B, H, Lq]: sum_d dout o
+  unsigned* grad_top;    // bits of the largest |dout| (fp16) or null
   void* dq;              // [B, Lq, H, D]
   void* dk; void* dv;    // [B, Lk, Hk, D]
 };
@@ -162,11 +162,10 @@ DEVINL void forward_row(const AttnArgs& a, int b, int i, int h) {
 }
 
 template <typename T>
-DEVINL void dq_row(const AttnArgs& a, int b, int i, int h) {
+DEVINL void dq_row(const AttnArgs& a, int b, int i, int h, float delta) {
   const int lane = threadIdx.x % WAVE, c = h / (a.H / a.Hk), at = i + a.Lk - a.Lq;
   const float slope = a.slopes != nullptr ? a.slopes[h] : 0.f;
-  const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.Lq + i;
-  const float lse = a.lse[stat], delta = a.delta[stat];
+  const float lse = a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + i];
   const T* q = q_row<T>(a, b, i, h);
   const T* g = g_row<T>(a, b, i, h);
   float dq[2] = {0.f, 0.f};

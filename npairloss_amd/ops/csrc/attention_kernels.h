@@ -29,37 +29,44 @@ DEVINL Query query_of(const AttnArgs& a, int b, int i, int h, bool ok) {
 }
 
 // What scores go through, as a constant of the kernel, so that products and
-// exponentials are one block of instructions: nothing (one factor, not zero); the
-// cap; a bias with or without the cap, or a factor of zero.
-enum Score { kPlain, kCapped, kBiased };
+// exponentials are one block of instructions: nothing (one factor, not zero), the
+// cap, a bias (or a factor of zero), both.
+enum Score { kPlain, kCapped, kBiased, kBoth };
+constexpr bool capped(Score s) { return s == kCapped || s == kBoth; }
 
-// Scores in registers to base-2 scores: on return a score is s * (the returned
-// factor).  Lanes are queries and registers keys: `first` is the key of register 0
-// of half 0.  `bend`: the cap's derivative, for the backward pass.
-template <typename T, Score SC, bool BEND>
-DEVINL float transform(const AttnArgs& a, f32x16& s, f32x16* bend, int first, int at, float slope2) {
-  const float c = fabsf(a.scale) * kLog2e;
-  if (SC == kPlain) return c;
-  const int half = threadIdx.x % WAVE / 32;
-  if (SC == kCapped || a.softcap > 0.f) {
-    const float in = fabsf(a.scale) / a.softcap, out = a.softcap * kLog2e;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float u = cap_share<T>(s[r] * in);
-      s[r] = fmaf(-2.f * out, u, out);
-      if (BEND) (*bend)[r] = 4.f * fmaf(-u, u, u);
+// A score in a register to one in base 2 (a kPlain one still wants the factor).
+// Lanes are queries and registers keys, or the other way round: only the distance
+// matters.
+template <typename T, Score SC>
+struct ScoreMap {
+  float factor;  // of the exponent's argument
+  float in, out, slope2, d0;
+
+  // `apart`: what the lane's index is ahead of the first register's of half 0.
+  DEVINL ScoreMap(const AttnArgs& a, float slope, int apart) {
+    const float c = fabsf(a.scale) * kLog2e;
+    factor = SC == kPlain ? c : 1.f;
+    in = capped(SC) ? fabsf(a.scale) / a.softcap : c;
+    out = a.softcap * kLog2e;
+    slope2 = slope;
+    d0 = static_cast<float>(apart - 4 * (static_cast<int>(threadIdx.x) % WAVE / 32));
+  }
+
+  // Register r; `bend` gets the cap's derivative.
+  DEVINL float operator()(float s, int r, float& bend) const {
+    bend = 1.f;
+    if (SC == kPlain) return s;
+    if (capped(SC)) {
+      const float u = cap_share<T>(s * in);
+      bend = 4.f * fmaf(-u, u, u);
+      s = fmaf(-2.f * out, u, out);
+    } else {
+      s *= in;
     }
-  } else {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= c;
+    if (SC == kBiased || SC == kBoth) s -= slope2 * fabsf(d0 - static_cast<float>(result_row(r, 0)));
+    return s;
   }
-  if (SC == kBiased) {
-    const float d0 = static_cast<float>(at - first - 4 * half);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] -= slope2 * fabsf(d0 - static_cast<float>(result_row(r, 0)));
-  }
-  return 1.f;
-}
+};
 
 // Which registers a query sees, as bits.
 DEVINL uint32_t seen_keys(const AttnArgs& a, const Query& q, const int* kd, int first, int row0) {
@@ -108,33 +115,31 @@ struct Online {
     outputs(at, vs, p);
   }
 
-  DEVINL void scores(const Reader<T, DP>& at, const Frag<T> (&qf)[DP / 16], const T* ks, f32x16 (&s)[NS]) {
+  static DEVINL void scores(const Reader<T, DP>& at, const Frag<T> (&qf)[DP / 16], const T* ks, f32x16 (&s)[NS]) {
+    constexpr int kSteps = DP / 16;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      s[n] = zeros16();
-#pragma unroll
-      for (int step = 0; step < DP / 16; ++step) product(at.rows(ks, 32 * n, step), qf[step], s[n]);
-    }
-    paced<T, NS * DP / 16, 1, 4>();
+    for (int n = 0; n < NS; ++n) s[n] = zeros16();
+    piped<T, NS * kSteps, 4>([&](auto i) { return at.rows(ks, 32 * (i / kSteps), i % kSteps); },
+                             [&](auto i, const Frag<T>& k) { product(k, qf[i % kSteps], s[i / kSteps]); });
   }
 
   template <Score SC, bool MASKED>
   DEVINL void weights(const AttnArgs& a, f32x16 (&s)[NS], Frag<T> (&p)[NS][2], const int* kd, const Query& q, int first) {
     float c = 1.f, high = -INFINITY;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) c = transform<T, SC, false>(a, s[n], nullptr, first + 32 * n, q.at, q.slope2);
-    if (MASKED) {
+    for (int n = 0; n < NS; ++n) {
+      const ScoreMap<T, SC> map(a, q.slope2, q.at - first - 32 * n);
+      c = map.factor;
+      uint32_t seen = 0xFFFF;
+      if (MASKED) seen = seen_keys(a, q, kd, first + 32 * n, 32 * n);
 #pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        const uint32_t seen = seen_keys(a, q, kd, first + 32 * n, 32 * n);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] = (seen >> r & 1) ? s[n][r] : -INFINITY;
+      for (int r = 0; r < 16; ++r) {
+        float bend;
+        s[n][r] = map(s[n][r], r, bend);
+        if (MASKED) s[n][r] = (seen >> r & 1) ? s[n][r] : -INFINITY;
+        high = fmaxf(high, s[n][r]);
       }
     }
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) high = fmaxf(high, s[n][r]);
     high = fmaxf(high, other_half(high)) * c;
     const float now = fmaxf(top, high), from = now == -INFINITY ? 0.f : now;
     const float keep = __builtin_amdgcn_exp2f(top - from);
@@ -147,22 +152,17 @@ struct Online {
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -from));
-        l += w;
-        p[n][r / 8].set(r % 8, w);
+      for (int r = 0; r < 16; r += 2) {
+        const float w0 = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -from)), w1 = __builtin_amdgcn_exp2f(fmaf(s[n][r + 1], c, -from));
+        l += w0 + w1;
+        p[n][r / 8].set2(r % 8, w0, w1);
       }
   }
 
   DEVINL void outputs(const Reader<T, DP>& at, const T* vs, const Frag<T> (&p)[NS][2]) {
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int x = 0; x < DP / 32; ++x) product(at.columns(vs, 32 * n + 16 * t, x), p[n][t], o[x]);
-    paced<T, NS * DP / 16, 2, 4>();
+    constexpr int kWide = DP / 32;
+    piped<T, NS * 2 * kWide, 4>([&](auto i) { return at.columns(vs, 16 * (i / kWide), i % kWide); },
+                                [&](auto i, const Frag<T>& v) { product(v, p[i / kWide / 2][i / kWide % 2], o[i % kWide]); });
   }
 };
 
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
   auto load = [&](int j, auto buf) {
     there = first_rows(a.Lk - j);
     if (own != nullptr) {
-      range_next = own[j / kDocTile];
+      range_next = walk.of(j / kDocTile);
       there = range_next.there >> (j % kDocTile);
       ids = staged_word(d0 + j, t, min(KT, a.Lk - j));
     }
@@ -531,21 +531,17 @@ __global__ __launch_bounds__(kThreads) void join_splits_kernel(AttnArgs a, int s
 
 // fp16 has 2^-14 for its least normal number, and over long rows weights and score
 // gradients lie under it.  Weights are taken times 2^10 in the products over
-// queries; score gradients times a power of two that brings the largest |dO|
-// (found with delta) to 1/4 .. 1/2, so that they overflow only where a sum over the
-// width is over 2^17 times that, and then the row is done again.
-template <typename T>
-DEVINL float grad_scale(const AttnArgs& a) {
-  if (!std::is_same<T, fp16_t>::value) return 1.f;
-  const float top = __uint_as_float(*a.grad_top);
-  return top > 0.f ? exp2f(-static_cast<float>(ilogbf(top)) - 2.f) : 1.f;
-}
+// queries; score gradients times a power of two that brings the largest |dO| (of the
+// query for dQ, of all for dK) to 1/4 .. 1/2, so that they overflow only where a sum
+// over the width is over 2^17 times that, and then the row is done again.
+DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(-static_cast<float>(ilogbf(top)) - 2.f) : 1.f; }
 
-// dQ of 32 queries a wave: lanes are queries, K and V pass by in tiles.
+// dQ of 32 queries a wave, and delta for both: lanes are queries, K and V pass by in
+// tiles.
 //   P^T = 2^(S^T - lse), dS^T = P^T (V dO^T - delta) bend, dQ^T += K^T dS^T
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
-  constexpr int KT = sizeof(T) == 2 ? 64 : 32;
+  constexpr int KT = sizeof(T) == 2 && DP == 64 ? 64 : 32;
   __shared__ __attribute__((aligned(16))) T ks[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T vs[2][KT * DP];
   __shared__ __attribute__((aligned(16))) int kd[2][KT];
@@ -565,9 +561,35 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
 #pragma unroll
     for (int x = 0; x < DP / 16; ++x) qf[x].v = -qf[x].v;
   }
+  // delta = sum_d dO o, with what o's rounding left: it is subtracted from every dP of a
+  // row, so that its error does not average out, and with o in 16 bits it was the
+  // largest in dQ and dK.
+  float delta = 0.f, high = 0.f;
+  {
+    const int64_t row = ((static_cast<int64_t>(b) * a.Lq + (ok ? i : 0)) * a.H + h) * a.D;
+    Frag<T> of[DP / 16], rest[DP / 16];
+    load_operands<T, DP>(static_cast<const T*>(a.o) + row, ok, a.D, of);
+    load_operands<T, DP>(static_cast<const T*>(a.o_rest) + row, ok && a.o_rest != nullptr, a.D, rest);
+#pragma unroll
+    for (int x = 0; x < DP / 16; ++x)
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const float g = to_f(gf[x].v[y]);
+        delta = fmaf(g, to_f(of[x].v[y]) + to_f(rest[x].v[y]), delta);
+        if (std::is_same<T, fp16_t>::value && fabsf(g) <= FLT_MAX) high = fmaxf(high, fabsf(g));
+      }
+    delta += other_half(delta);
+    if (ok && lane < 32) a.delta[bh * a.Lq + i] = delta;
+  }
   // dS of fp16 is scaled into its range (see grad_scale), through the exponent
-  const float lift = grad_scale<T>(a);
-  const float lse = ok ? a.lse[bh * a.Lq + i] - log2f(lift) : INFINITY, delta = ok ? a.delta[bh * a.Lq + i] : 0.f;
+  float lift = 1.f;
+  if constexpr (std::is_same<T, fp16_t>::value) {
+    lift = grad_scale(fmaxf(high, other_half(high)));
+    high = wave_reduce_max(high);  // a maximum does not depend on the order it is taken in
+    if (lane == 0 && __float_as_uint(high) > __hip_atomic_load(a.grad_top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+      atomicMax(a.grad_top, __float_as_uint(high));
+  }
+  const float lse = ok ? a.lse[bh * a.Lq + i] - log2f(lift) : INFINITY;
   // rows that are not there decide nothing, and nothing of them is kept
   const int least_end = wave_min(ok ? q.end : INT_MAX), most_end = wave_max(q.end);
   const int doc_lo = wave_min(ok ? q.doc : INT_MAX), doc_hi = wave_max(ok ? q.doc : INT_MIN);
@@ -607,33 +629,64 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
 #pragma unroll
   for (int x = 0; x < DP / 32; ++x) dq[x] = zeros16();
   const Reader<T, DP> reader;
+  // With registers for two sets, the scores of 32 keys pass under the weights of the 32
+  // before, and those' products under the weights of these; with one, the other wave
+  // of the SIMD has to fill the time.
+  constexpr int kSub = KT / 32, kSteps = DP / 16, kWide = DP / 32;
   auto step = [&](auto masked, int j, auto buf) {
     const Reader<T, DP> at = reader.fresh();
+    f32x16 s[kSub], dp[kSub];
+    Frag<T> ds[kSub][2];
+    auto score = [&](int n, int i, const Frag<T>& f) {
+      if (i == 0) s[n] = zeros16(), dp[n] = zeros16();
+      if (i % 2 == 0) product(f, qf[i / 2], s[n]);
+      else product(f, gf[i / 2], dp[n]);
+    };
+    auto score_read = [&](int n, int i) { return at.rows(i % 2 == 0 ? ks[buf] : vs[buf], 32 * n, i / 2); };
+    auto output = [&](int n, int i, const Frag<T>& f) { product(f, ds[n][i / kWide], dq[i % kWide]); };
+    auto output_read = [&](int n, int i) { return at.columns(ks[buf], 32 * n + 16 * (i / kWide), i % kWide); };
+    uint32_t seen[kSub];
+    auto weight = [&](int n, int r) {  // registers r and r + 1
+      const ScoreMap<T, SC> map(a, q.slope2, q.at - j - 32 * n);
+      if (masked && r == 0) seen[n] = seen_keys(a, q, kd[buf], j + 32 * n, 32 * n);
+      float x[2];
 #pragma unroll
-    for (int n = 0; n < KT / 32; ++n) {
-      f32x16 s = zeros16(), dp = zeros16(), bend;
-#pragma unroll
-      for (int x = 0; x < DP / 16; ++x) {
-        product(at.rows(ks[buf], 32 * n, x), qf[x], s);
-        product(at.rows(vs[buf], 32 * n, x), gf[x], dp);
+      for (int y = 0; y < 2; ++y) {
+        float bend;
+        const float t = map(s[n][r + y], r + y, bend);
+        x[y] = __builtin_amdgcn_exp2f(fmaf(t, map.factor, -lse)) * (dp[n][r + y] - delta);
+        if (capped(SC)) x[y] *= bend;
+        if (masked) x[y] = (seen[n] >> (r + y) & 1) ? x[y] : 0.f;
       }
-      paced<T, DP / 8, 1, 4>();
-      const float c = transform<T, SC, true>(a, s, &bend, j + 32 * n, q.at, q.slope2);
-      uint32_t seen = 0xFFFF;
-      if (masked) seen = seen_keys(a, q, kd[buf], j + 32 * n, 32 * n);
-      Frag<T> ds[2];
+      ds[n][r / 8].set2(r % 8, x[0], x[1]);
+    };
+    constexpr int kA = 2 * kSteps, kB = 2 * kWide;  // products of scores and of outputs
+    if constexpr (kSub == 2 && DP == 64) {
+      piped<T, 2 * kA + 2 * kB, 4>(
+          [&](auto i) { return i < 2 * kA ? score_read(i / kA, i % kA) : output_read((i - 2 * kA) / kB, (i - 2 * kA) % kB); },
+          [&](auto i, const Frag<T>& f) {
+            if (i < kA) {
+              score(0, i, f);
+            } else if (i < 2 * kA) {
+              score(1, i - kA, f);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float x = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
-        if (SC == kCapped || (SC == kBiased && a.softcap > 0.f)) x *= bend[r];
-        ds[r / 8].set(r % 8, !masked || (seen >> r & 1) ? x : 0.f);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+              for (int r = 16 / kA * (i - kA); r < 16 / kA * (i - kA + 1); r += 2) weight(0, r);
+            } else if (i < 2 * kA + kB) {
+              output(0, i - 2 * kA, f);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+              for (int r = 16 / kB * (i - 2 * kA); r < 16 / kB * (i - 2 * kA + 1); r += 2) weight(1, r);
+            } else {
+              output(1, i - 2 * kA - kB, f);
+            }
+          });
+    } else {
+      each(std::make_integer_sequence<int, kSub>(), [&](auto n) {
+        piped<T, kA, 4>([&](auto i) { return score_read(n, i); }, [&](auto i, const Frag<T>& f) { score(n, i, f); });
 #pragma unroll
-        for (int x = 0; x < DP / 32; ++x) product(at.columns(ks[buf], 32 * n + 16 * u, x), ds[u], dq[x]);
-      paced<T, DP / 16, 2, 4>();
+        for (int r = 0; r < 16; r += 2) weight(n, r);
+        __builtin_amdgcn_sched_barrier(0);
+        piped<T, kB, 4>([&](auto i) { return output_read(n, i); }, [&](auto i, const Frag<T>& f) { output(n, i, f); });
+      });
     }
   };
   uint32_t ids = 0;
@@ -642,7 +695,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   auto load = [&](int j, auto buf) {
     there = first_rows(a.Lk - j);
     if (own != nullptr) {
-      range_next = own[j / kDocTile];
+      range_next = walk.of(j / kDocTile);
       there = range_next.there >> (j % kDocTile);
       ids = staged_word(d0 + j, t, min(KT, a.Lk - j));
     }
@@ -684,7 +737,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   if (repairs<T>(a)) again = bad_columns(ok && !finite_column(dq));
   if (ok && !(again >> (lane % 32) & 1))
     store_column<T, DP>(static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D, dq, a.D, a.scale / lift);
-  for (; again != 0; again &= again - 1) dq_row<T>(a, b, i0 + 32 * wave + __builtin_ctz(again), h);
+  for (; again != 0; again &= again - 1)
+    dq_row<T>(a, b, i0 + 32 * wave + __builtin_ctz(again), h, lane_of(delta, __builtin_ctz(again)));
 }
 
 // dK and dV of 32 keys a wave: lanes are keys, Q and dO of all heads that share
@@ -702,7 +756,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
   const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
   const int split = linear % splits;
   const int64_t bc = linear / splits / k_blocks;
-  const int j0 = static_cast<int>(linear / splits % k_blocks) * kKeys;
+  // first, last, second, ..: a causal mask leaves the first blocks the most queries, and
+  // an XCD has a stretch of this order
+  const int place = static_cast<int>(linear / splits % k_blocks);
+  const int j0 = (place % 2 == 0 ? place / 2 : k_blocks - 1 - place / 2) * kKeys;
   const int b = bc / a.Hk, kv = bc % a.Hk, group = a.H / a.Hk, off = a.Lk - a.Lq;
   const int j = j0 + 32 * wave + lane % 32;
   const int doc = j < a.Lk && a.k_doc != nullptr ? a.k_doc[static_cast<int64_t>(b) * a.Lk + j] : 0;
@@ -767,69 +824,98 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
     return n * kDocTile;
   };
   constexpr float kWeightLift = sizeof(T) == 2 && std::is_same<T, fp16_t>::value ? 10.f : 0.f;  // see grad_scale
-  const float lift = grad_scale<T>(a);
+  float lift = 1.f;
+  if constexpr (std::is_same<T, fp16_t>::value) lift = grad_scale(__uint_as_float(*a.grad_top));
   const int* d0 = a.q_doc != nullptr ? a.q_doc + static_cast<int64_t>(b) * a.Lq : nullptr;
 
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int x = 0; x < DP / 32; ++x) dk[x] = zeros16(), dv[x] = zeros16();
   const Reader<T, DP> reader;
-  auto step = [&](auto masked, int i, float slope2, auto buf) {
+  // The scores of 32 queries pass under the weights of the 32 before, and those'
+  // products under the weights of these.
+  constexpr int kSub = QT / 32, kSteps = DP / 16, kWide = DP / 32;
+  auto step = [&](auto masked, int i0, float slope2, auto buf) {
     const Reader<T, DP> at = reader.fresh();
-#pragma unroll
-    for (int n = 0; n < QT / 32; ++n) {
-      f32x16 s = zeros16(), dp = zeros16(), bend;
-#pragma unroll
-      for (int x = 0; x < DP / 16; ++x) {
-        product(at.rows(qs[buf], 32 * n, x), kf[x], s);
-        product(at.rows(gs[buf], 32 * n, x), vf[x], dp);
-      }
-      paced<T, DP / 8, 1, 4>();
+    f32x16 s[kSub], dp[kSub];
+    Frag<T> p[kSub][2], ds[kSub][2];
+    auto score = [&](int n, int i, const Frag<T>& f) {
+      if (i == 0) s[n] = zeros16(), dp[n] = zeros16();
+      if (i % 2 == 0) product(f, kf[i / 2], s[n]);
+      else product(f, vf[i / 2], dp[n]);
+    };
+    auto score_read = [&](int n, int i) { return at.rows(i % 2 == 0 ? qs[buf] : gs[buf], 32 * n, i / 2); };
+    auto output = [&](int n, int i, const Frag<T>& f) {
+      if (i % 2 == 0) product(f, p[n][i / 2 / kWide], dv[i / 2 % kWide]);
+      else product(f, ds[n][i / 2 / kWide], dk[i / 2 % kWide]);
+    };
+    auto output_read = [&](int n, int i) { return at.columns(i % 2 == 0 ? gs[buf] : qs[buf], 32 * n + 16 * (i / 2 / kWide), i / 2 % kWide); };
+    uint32_t seen[kSub];
+    float4 lse, del;
+    auto weight = [&](int n, int r) {  // registers r and r + 1
       // the distance |i + off - j| with queries in registers: as if the key stood at j - off
-      const float c = transform<T, SC, true>(a, s, &bend, i + 32 * n, j - off, slope2);
-      uint32_t seen = 0xFFFF;
-      if (masked) {
-        seen = 0;
-        const int from = begin == INT_MAX ? INT_MAX : begin - i - 32 * n - 4 * half;
+      const ScoreMap<T, SC> map(a, slope2, j - off - i0 - 32 * n);
+      if (masked && r == 0) {
+        seen[n] = 0;
+        const int from = begin == INT_MAX ? INT_MAX : begin - i0 - 32 * n - 4 * half;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) seen |= static_cast<uint32_t>(result_row(r, 0) >= from) << r;
+        for (int x = 0; x < 16; ++x) seen[n] |= static_cast<uint32_t>(result_row(x, 0) >= from) << x;
         if (own != nullptr) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int4 d = *reinterpret_cast<const int4*>(&qd[buf][32 * n + 8 * x + 4 * half]);
             const uint32_t same = static_cast<uint32_t>(d.x == doc) | static_cast<uint32_t>(d.y == doc) << 1 |
                                   static_cast<uint32_t>(d.z == doc) << 2 | static_cast<uint32_t>(d.w == doc) << 3;
-            seen &= same << (4 * x) | ~(15u << (4 * x));
+            seen[n] &= same << (4 * x) | ~(15u << (4 * x));
           }
         }
       }
-      Frag<T> p[2], ds[2];
+      if (r % 4 == 0) {
+        lse = *reinterpret_cast<const float4*>(&stats[buf][0][32 * n + 2 * r + 4 * half]);
+        del = *reinterpret_cast<const float4*>(&stats[buf][1][32 * n + 2 * r + 4 * half]);
+      }
+      const float ls[2] = {r % 4 == 0 ? lse.x : lse.z, r % 4 == 0 ? lse.y : lse.w}, de[2] = {r % 4 == 0 ? del.x : del.z, r % 4 == 0 ? del.y : del.w};
+      float w[2], g[2];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float4 lse = *reinterpret_cast<const float4*>(&stats[buf][0][32 * n + 8 * x + 4 * half]);
-        const float4 del = *reinterpret_cast<const float4*>(&stats[buf][1][32 * n + 8 * x + 4 * half]);
-        const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {del.x, del.y, del.z, del.w};
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int r = 4 * x + y;
-          const float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, -ls[y]));
-          float g = w * (dp[r] - de[y]);
-          if (SC == kCapped || (SC == kBiased && a.softcap > 0.f)) g *= bend[r];
-          if (std::is_same<T, fp16_t>::value) g *= lift;
-          const bool sees = !masked || (seen >> r & 1);
-          p[r / 8].set(r % 8, sees ? w : 0.f);
-          ds[r / 8].set(r % 8, sees ? g : 0.f);
+      for (int y = 0; y < 2; ++y) {
+        float bend;
+        const float t = map(s[n][r + y], r + y, bend);
+        w[y] = __builtin_amdgcn_exp2f(fmaf(t, map.factor, -ls[y]));
+        g[y] = w[y] * (dp[n][r + y] - de[y]);
+        if (capped(SC)) g[y] *= bend;
+        if (std::is_same<T, fp16_t>::value) g[y] *= lift;
+        if (masked) {
+          const bool sees = seen[n] >> (r + y) & 1;
+          w[y] = sees ? w[y] : 0.f;
+          g[y] = sees ? g[y] : 0.f;
         }
       }
+      p[n][r / 8].set2(r % 8, w[0], w[1]);
+      ds[n][r / 8].set2(r % 8, g[0], g[1]);
+    };
+    constexpr int kA = 2 * kSteps, kB = 4 * kWide;  // products of scores and of outputs: as many
+    static_assert(kA == kB && 16 % kA == 0, "pairs of registers go by products");
+    constexpr int kRows = 16 / kA < 2 ? 2 : 16 / kA, kEvery = kA / (16 / kRows);  // rows at every so many products
+    auto weights_beside = [&](int n, int i) {
+      if (i % kEvery == 0)
+#pragma unroll
+        for (int r = kRows * (i / kEvery); r < kRows * (i / kEvery + 1); r += 2) weight(n, r);
+    };
+    if constexpr (kSub == 2) {
+      piped<T, 4 * kA, 4>(
+          [&](auto i) { return i < 2 * kA ? score_read(i / kA, i % kA) : output_read(i / kA - 2, i % kA); },
+          [&](auto i, const Frag<T>& f) {
+            if (i < 2 * kA) score(i / kA, i % kA, f);
+            else output(i / kA - 2, i % kA, f);
+            if (i / kA == 1) weights_beside(0, i % kA);
+            if (i / kA == 2) weights_beside(1, i % kA);
+          });
+    } else {
+      piped<T, kA, 4>([&](auto i) { return score_read(0, i); }, [&](auto i, const Frag<T>& f) { score(0, i, f); });
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) weight(0, r);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int x = 0; x < DP / 32; ++x) {
-          product(at.columns(gs[buf], 32 * n + 16 * u, x), p[u], dv[x]);
-          product(at.columns(qs[buf], 32 * n + 16 * u, x), ds[u], dk[x]);
-        }
-      paced<T, DP / 8, 2, 4>();
+      piped<T, kB, 4>([&](auto i) { return output_read(0, i); }, [&](auto i, const Frag<T>& f) { output(0, i, f); });
     }
   };
   uint32_t ids = 0, stat = 0;
@@ -841,7 +927,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
     const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.Lq + i;
     stat = staged_word((wave == 0 ? a.lse : a.delta) + row, lane, wave < 2 ? rows : 0);  // one wave brings lse, one delta
     if (own != nullptr) {
-      range_next = own[i / kDocTile];
+      range_next = walk.of(i / kDocTile);
       there = range_next.there >> (i % kDocTile);
       ids = staged_word(d0 + i, t, rows);
     }
@@ -931,50 +1017,6 @@ __global__ __launch_bounds__(kThreads) void join_dkv_kernel(AttnArgs a, int spli
     }
 }
 
-// delta[b, h, i] = sum_d dout o: sixteen lanes a row.  o is taken with what its
-// rounding left: delta is subtracted from every dP of a row, so that its error does
-// not average out, and with o in 16 bits it was the largest in dQ and dK.
-// `top`: the bits of the largest finite |dout|, or null: a maximum does not depend on
-// the order it is taken in, and a workgroup brings one.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void delta_kernel(AttnArgs a, float* __restrict__ delta, unsigned* __restrict__ top, int64_t rows) {
-  __shared__ float highs[kWaves];
-  const int t = threadIdx.x % 16;
-  float high = 0.f;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + threadIdx.x / 16; row < rows;
-       row += static_cast<int64_t>(gridDim.x) * (kThreads / 16)) {
-    const int64_t bl = row / a.H;
-    const int h = row % a.H, b = bl / a.Lq, i = bl % a.Lq;
-    const T* g = g_row<T>(a, b, i, h);
-    const T* o = static_cast<const T*>(a.o) + row * a.D;
-    float s = 0.f;
-    if (t * 8 < a.D) {
-      float x[8], y[8];
-      load8(g + t * 8, x);
-      load8(o + t * 8, y);
-      if (a.o_rest != nullptr) {
-        float rest[8];
-        load8(static_cast<const T*>(a.o_rest) + row * a.D + t * 8, rest);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] += rest[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        s = fmaf(x[e], y[e], s);
-        if (fabsf(x[e]) <= FLT_MAX) high = fmaxf(high, fabsf(x[e]));
-      }
-    }
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor(s, off, 16);  // sixteen lanes leave the loop together
-    if (t == 0) delta[(static_cast<int64_t>(b) * a.H + h) * a.Lq + i] = s;
-  }
-  if (top == nullptr) return;
-  high = wave_reduce_max(high);
-  if (threadIdx.x % WAVE == 0) highs[threadIdx.x / WAVE] = high;
-  __syncthreads();
-  if (threadIdx.x == 0) atomicMax(top, __float_as_uint(fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3]))));
-}
-
 int blocks_for(int64_t items, int64_t each) {
   const int64_t n = (items + each - 1) / each;
   TORCH_CHECK(n < (int64_t{1} << 31), "attention: too many rows");
@@ -987,7 +1029,9 @@ constexpr int kComputeUnits = 256;
 template <typename Fn>
 void with_variant(const AttnArgs& a, Fn fn) {
   auto by_score = [&](auto width) {
-    if (a.slopes != nullptr || a.scale == 0.f) fn(width, std::integral_constant<Score, kBiased>());
+    const bool biased = a.slopes != nullptr || a.scale == 0.f;
+    if (biased && a.softcap > 0.f) fn(width, std::integral_constant<Score, kBoth>());
+    else if (biased) fn(width, std::integral_constant<Score, kBiased>());
     else if (a.softcap > 0.f) fn(width, std::integral_constant<Score, kCapped>());
     else fn(width, std::integral_constant<Score, kPlain>());
   };
@@ -1052,9 +1096,6 @@ void attention_forward(const AttnArgs& a, const DocRange* ranges, const torch::T
 template <typename T>
 void attention_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q_ranges, const torch::TensorOptions& options,
                         hipStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.B) * a.H * a.Lq;
-  delta_kernel<T><<<std::min(blocks_for(rows, kThreads / 16), 8 * kComputeUnits), kThreads, 0, stream>>>(
-      a, const_cast<float*>(a.delta), const_cast<unsigned*>(a.grad_top), rows);
   with_variant(a, [&](auto width, auto score) {
     run_backward<T, decltype(width)::value, decltype(score)::value>(a, k_ranges, q_ranges, options, stream);
   });

@@ -21,25 +21,23 @@
 
 #include "attention.h"
 
+#include <utility>
+
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 using u32x4 = __attribute__((ext_vector_type(4))) unsigned int;
 
-template <typename T> struct Frag;  // eight k of one row or column
-template <> struct Frag<bf16_t> {
-  using V = __attribute__((ext_vector_type(8))) bf16_t;
+template <typename T>
+struct Frag {  // eight k of one row or column
+  using V = __attribute__((ext_vector_type(8))) T;
   V v;
-  DEVINL void set(int i, float x) { v[i] = static_cast<bf16_t>(x); }
-};
-template <> struct Frag<fp16_t> {
-  using V = __attribute__((ext_vector_type(8))) fp16_t;
-  V v;
-  DEVINL void set(int i, float x) { v[i] = static_cast<fp16_t>(x); }
-};
-template <> struct Frag<float> {
-  using V = __attribute__((ext_vector_type(8))) float;
-  V v;
-  DEVINL void set(int i, float x) { v[i] = x; }
+  DEVINL void set2(int i, float x, float y) {  // one conversion for two
+    using F2 = __attribute__((ext_vector_type(2))) float;
+    using T2 = __attribute__((ext_vector_type(2))) T;
+    const T2 t = __builtin_convertvector((F2{x, y}), T2);
+    v[i] = t[0];
+    v[i + 1] = t[1];
+  }
 };
 
 DEVINL void product(const Frag<bf16_t>& a, const Frag<bf16_t>& b, f32x16& c) {
@@ -53,22 +51,26 @@ DEVINL void product(const Frag<float>& a, const Frag<float>& b, f32x16& c) {
   for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
 }
 
-// The order of a block of N products and the reads of shared memory that bring one
-// operand of each (READS instructions): AHEAD operands first, then a product for
-// every further one, so that a read's latency passes under products, and no more
-// registers are taken than that.  Nothing moves across its ends.
-template <typename T, int N, int READS, int AHEAD>
-DEVINL void paced() {
-  if constexpr (sizeof(T) == 2) {
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
-#pragma unroll
-    for (int i = 0; i < N - AHEAD; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
-  }
+// N products in a row, each with an operand from shared memory: `read(i)` brings it,
+// AHEAD of them before the first `use(i, operand)` and one more behind each, so that a
+// read's latency passes under products and under what else `use` does.  The compiler
+// left alone waits for every read in front of its product; the barriers hold the
+// order as it is written.
+template <typename Fn, int... I>
+DEVINL void each(std::integer_sequence<int, I...>, Fn fn) {
+  (fn(std::integral_constant<int, I>()), ...);
+}
+
+template <typename T, int N, int AHEAD, typename Read, typename Use>
+DEVINL void piped(Read read, Use use) {
+  Frag<T> f[AHEAD];
+  each(std::make_integer_sequence<int, AHEAD>(), [&](auto i) { f[i] = read(i); });
   __builtin_amdgcn_sched_barrier(0);
+  each(std::make_integer_sequence<int, N>(), [&](auto i) {
+    use(i, f[i % AHEAD]);
+    if constexpr (i + AHEAD < N) f[i % AHEAD] = read(std::integral_constant<int, i + AHEAD>());
+    __builtin_amdgcn_sched_barrier(0);
+  });
 }
 
 DEVINL f32x16 zeros16() {
@@ -118,6 +120,11 @@ struct Reader {
     Reader r = *this;
     asm volatile("" : "+v"(r.row_at), "+v"(r.col_at));
     return r;
+  }
+
+  DEVINL void move(int rows) {  // by a multiple of 16
+    row_at += rows * DP;
+    col_at += rows * DP;
   }
 
   // Row row0 + lane % 32 (row0 a multiple of 16), k = 16 step + 8 half ...: an
@@ -242,16 +249,18 @@ struct DocRange {
 };
 constexpr int kDocTile = 64;
 
-// Which tiles of 64 rows an interval of ids may meet: 64 of them at a time.
+// Which tiles of 64 rows an interval of ids may meet: 64 of them at a time, a lane
+// holds one's ids.
 struct TileWalk {
   const DocRange* ranges;  // or null: all
   int lo, hi;              // ids on the other side
   int next_base, end;      // tiles [.., end)
   uint64_t bits;
   int base;
+  DocRange mine;           // of tile base + lane
 
   DEVINL TileWalk(const DocRange* r, int lo_, int hi_, int begin, int end_)
-      : ranges(r), lo(lo_), hi(hi_), next_base(begin), end(end_), bits(0), base(begin) {}
+      : ranges(r), lo(lo_), hi(hi_), next_base(begin), end(end_), bits(0), base(begin), mine{0, 0, 0} {}
 
   // The next tile, or -1.  All lanes of the wave together.
   DEVINL int next() {
@@ -261,11 +270,23 @@ struct TileWalk {
       next_base += 64;
       const int t = base + threadIdx.x % WAVE;
       bool meets = t < end;
-      if (ranges != nullptr && meets) meets = ranges[t].lo <= hi && ranges[t].hi >= lo;
+      if (ranges != nullptr && meets) {
+        mine = ranges[t];
+        meets = mine.lo <= hi && mine.hi >= lo;
+      }
       bits = __ballot(meets);
     }
     const int t = base + __builtin_ctzll(bits);
     bits &= bits - 1;
     return t;
+  }
+
+  // The ids of a tile that next() gave since it last took 64.
+  DEVINL DocRange of(int tile) const {
+    const int lane = tile - base;
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine.there), lane);
+    const uint32_t high = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine.there >> 32), lane);
+    return DocRange{__builtin_amdgcn_readlane(mine.lo, lane), __builtin_amdgcn_readlane(mine.hi, lane),
+                    static_cast<uint64_t>(high) << 32 | low};
   }
 };
