@@ -60,6 +60,32 @@ def adamw_state(param: torch.Tensor, *, bits: int = 32, master: bool = False) ->
     return state
 
 
+def _check(params, grads, exp_avgs, exp_avg_sqs, steps, masters, scales) -> List[torch.Tensor]:
+    """The gradients, in the order of their parameters in memory."""
+    device, dtype = params[0].device, params[0].dtype
+    if dtype not in _FLOATS:
+        raise TypeError(f"adamw_step: fp32, bf16 or fp16 parameters expected, got {dtype}")
+    state = _FP8 if scales is not None else torch.float32
+    laid: List[torch.Tensor] = []
+    for i, (p, g, m, v, t) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, steps)):
+        if p.device != device or p.dtype != dtype:
+            raise ValueError(f"adamw_step: parameter {i} is {p.dtype} on {p.device}, the first {dtype} on {device}")
+        if not _dense(p):
+            raise ValueError(f"adamw_step: parameter {i} does not fill a stretch of memory (strides {p.stride()})")
+        if g.layout != torch.strided or g.shape != p.shape or g.dtype != dtype or g.device != device:
+            raise ValueError(f"adamw_step: gradient {i} {tuple(g.shape)} {g.dtype} does not fit {tuple(p.shape)} {dtype}")
+        for name, x, want in (("exp_avg", m, state), ("exp_avg_sq", v, state)) + ((("master", masters[i], torch.float32),) if masters is not None else ()):
+            if x.shape != p.shape or x.dtype != want or x.device != device or not _like(x, p):
+                raise ValueError(f"adamw_step: {name} {i} {tuple(x.shape)} {x.dtype} is not laid out as its parameter in {want}")
+        if t.numel() != 1 or t.dtype != torch.int32 or t.device != device:
+            raise ValueError(f"adamw_step: step {i} is one int32 on {device}")
+        if scales is not None and (scales[i].shape != ((p.numel() + BLOCK - 1) // BLOCK, 2) or scales[i].dtype != torch.float32
+                                   or scales[i].device != device or not scales[i].is_contiguous()):
+            raise ValueError(f"adamw_step: scales {i} {tuple(scales[i].shape)} are not fp32 [blocks of {BLOCK}, 2]")
+        laid.append(g if _like(g, p) else torch.empty_like(p).copy_(g))
+    return laid
+
+
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
                exp_avg_sqs: Sequence[torch.Tensor], steps: Sequence[torch.Tensor], *, lr: float,
                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -83,33 +109,13 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError(f"adamw_step: lr, eps and weight_decay are not negative, got {lr}, {eps}, {weight_decay}")
     if not len(params):
         return
-    device, dtype = params[0].device, params[0].dtype
-    if dtype not in _FLOATS:
-        raise TypeError(f"adamw_step: fp32, bf16 or fp16 parameters expected, got {dtype}")
-    state = _FP8 if scales is not None else torch.float32
-    laid: List[torch.Tensor] = []
-    for i, (p, g, m, v, t) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, steps)):
-        if p.device != device or p.dtype != dtype:
-            raise ValueError(f"adamw_step: parameter {i} is {p.dtype} on {p.device}, the first {dtype} on {device}")
-        if not _dense(p):
-            raise ValueError(f"adamw_step: parameter {i} does not fill a stretch of memory (strides {p.stride()})")
-        if g.layout != torch.strided or g.shape != p.shape or g.dtype != dtype or g.device != device:
-            raise ValueError(f"adamw_step: gradient {i} {tuple(g.shape)} {g.dtype} does not fit {tuple(p.shape)} {dtype}")
-        for name, x, want in (("exp_avg", m, state), ("exp_avg_sq", v, state)) + ((("master", masters[i], torch.float32),) if masters is not None else ()):
-            if x.shape != p.shape or x.dtype != want or x.device != device or not _like(x, p):
-                raise ValueError(f"adamw_step: {name} {i} {tuple(x.shape)} {x.dtype} is not laid out as its parameter in {want}")
-        if t.numel() != 1 or t.dtype != torch.int32 or t.device != device:
-            raise ValueError(f"adamw_step: step {i} is one int32 on {device}")
-        if scales is not None and (scales[i].shape != ((p.numel() + BLOCK - 1) // BLOCK, 2) or scales[i].dtype != torch.float32
-                                   or scales[i].device != device or not scales[i].is_contiguous()):
-            raise ValueError(f"adamw_step: scales {i} {tuple(scales[i].shape)} are not fp32 [blocks of {BLOCK}, 2]")
-        laid.append(g if _like(g, p) else torch.empty_like(p).copy_(g))
     with torch.no_grad():
-        if device.type == "cuda":
-            _backend.ext().adamw_update(list(params), laid, list(exp_avgs), list(exp_avg_sqs), list(steps), list(masters or ()),
+        if params[0].device.type == "cuda":  # checked there, as below
+            _backend.ext().adamw_update(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), list(steps), list(masters or ()),
                                         list(scales or ()), float(lr), float(betas[0]), float(betas[1]), float(eps),
                                         float(weight_decay), int(seed) & 0xFFFFFFFF)
             return
+        laid = _check(params, grads, exp_avgs, exp_avg_sqs, steps, masters, scales)
         for i, (p, g, m, v, t) in enumerate(zip(params, laid, exp_avgs, exp_avg_sqs, steps)):
             _step_torch(p, g, m, v, t, masters[i] if masters is not None else None, scales[i] if scales is not None else None,
                         lr, betas, eps, weight_decay, int(seed) & 0xFFFFFFFF, i)

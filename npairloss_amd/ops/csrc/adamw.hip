@@ -274,8 +274,9 @@ __global__ __launch_bounds__(kSteps) void raise_steps_kernel(StepArgs a) {
 
 }  // namespace
 
-// One step in place.  The lists go together; `masters` and `scales` are empty
-// or as long.  Tensors are dense and, list by list, laid out alike in memory.
+// One step in place.  The lists go together; `masters` and `scales` are empty or as
+// long.  Checked here and not in Python, where a hundred tensors take longer than
+// their step.
 void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> grads,
                   std::vector<torch::Tensor> ms, std::vector<torch::Tensor> vs,
                   std::vector<torch::Tensor> steps, std::vector<torch::Tensor> masters,
@@ -284,27 +285,40 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
   const size_t count = params.size();
   if (count == 0) return;
   const bool eight = !scales.empty();
-  TORCH_CHECK(grads.size() == count && ms.size() == count && vs.size() == count && steps.size() == count &&
-                  (masters.empty() || masters.size() == count) && (!eight || scales.size() == count),
-              "adamw_step: lists of different lengths");
+  TORCH_CHECK_VALUE(grads.size() == count && ms.size() == count && vs.size() == count && steps.size() == count &&
+                        (masters.empty() || masters.size() == count) && (!eight || scales.size() == count),
+                    "adamw_step: lists of different lengths");
   const auto device = params[0].device();
   const auto type = params[0].scalar_type();
-  TORCH_CHECK(device.is_cuda(), "adamw_step: GPU tensors expected");
+  TORCH_CHECK_TYPE(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf, "adamw_step: fp32, bf16 or fp16 parameters expected, got ", type);
   const auto state = eight ? at::kFloat8_e4m3fn : at::kFloat;
+  // whether elements of two tensors of one shape lie in memory in the same order
+  auto like = [](const torch::Tensor& x, const torch::Tensor& y) {
+    for (int64_t d = 0; d < y.dim(); ++d)
+      if (y.size(d) > 1 && x.stride(d) != y.stride(d)) return false;
+    return true;
+  };
   for (size_t i = 0; i < count; ++i) {
-    const int64_t n = params[i].numel();
-    auto fits = [&](const torch::Tensor& x, at::ScalarType want, int64_t numel) {
-      return x.device() == device && x.scalar_type() == want && x.numel() == numel &&
-             x.is_non_overlapping_and_dense();
+    const auto& p = params[i];
+    const int64_t n = p.numel();
+    auto fits = [&](const torch::Tensor& x, at::ScalarType want) {
+      return x.layout() == at::kStrided && x.device() == device && x.scalar_type() == want && x.sizes() == p.sizes();
     };
-    TORCH_CHECK(fits(params[i], type, n) && fits(grads[i], type, n) && fits(ms[i], state, n) && fits(vs[i], state, n),
-                "adamw_step: tensor ", i, ": parameter, gradient and moments do not go together");
-    TORCH_CHECK(fits(steps[i], at::kInt, 1), "adamw_step: tensor ", i, ": the step is one int32 on the device");
-    TORCH_CHECK(masters.empty() || fits(masters[i], at::kFloat, n), "adamw_step: tensor ", i, ": fp32 master expected");
-    TORCH_CHECK(!eight || (fits(scales[i], at::kFloat, (n + kBlock - 1) / kBlock * 2) && scales[i].is_contiguous() &&
-                           reinterpret_cast<uintptr_t>(scales[i].data_ptr()) % 8 == 0),
-                "adamw_step: tensor ", i, ": scales are fp32 [blocks of ", kBlock, ", 2]");
-    TORCH_CHECK(n < (int64_t{1} << 40), "adamw_step: tensor ", i, " is too large");
+    TORCH_CHECK_VALUE(fits(p, type) && p.is_cuda(), "adamw_step: parameter ", i, " is ", p.scalar_type(), " on ", p.device(),
+                      ", the first ", type, " on ", device);
+    TORCH_CHECK_VALUE(n == 0 || p.is_non_overlapping_and_dense(), "adamw_step: parameter ", i, " does not fill a stretch of memory");
+    TORCH_CHECK_VALUE(fits(grads[i], type), "adamw_step: gradient ", i, " does not fit its parameter");
+    TORCH_CHECK_VALUE(fits(ms[i], state) && like(ms[i], p) && fits(vs[i], state) && like(vs[i], p), "adamw_step: moments ", i,
+                      " are not laid out as their parameter in ", state);
+    TORCH_CHECK_VALUE(masters.empty() || (fits(masters[i], at::kFloat) && like(masters[i], p)), "adamw_step: master ", i,
+                      " is not laid out as its parameter in fp32");
+    TORCH_CHECK_VALUE(steps[i].device() == device && steps[i].scalar_type() == at::kInt && steps[i].numel() == 1, "adamw_step: step ", i,
+                      " is one int32 on ", device);
+    TORCH_CHECK_VALUE(!eight || (scales[i].device() == device && scales[i].scalar_type() == at::kFloat && scales[i].is_contiguous() &&
+                                 scales[i].dim() == 2 && scales[i].size(0) == (n + kBlock - 1) / kBlock && scales[i].size(1) == 2 &&
+                                 reinterpret_cast<uintptr_t>(scales[i].data_ptr()) % 8 == 0),
+                      "adamw_step: scales ", i, " are not fp32 [blocks of ", kBlock, ", 2]");
+    TORCH_CHECK_VALUE(n < (int64_t{1} << 40), "adamw_step: parameter ", i, " is too large");
   }
   for (const auto* list : {&params, &steps}) {  // a tensor that comes twice would be updated by two workgroups at once
     std::vector<const void*> at;
@@ -314,6 +328,8 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
     TORCH_CHECK(std::adjacent_find(at.begin(), at.end()) == at.end(), "adamw_step: a tensor comes twice");
   }
   at::DeviceGuard guard(device);
+  for (size_t i = 0; i < count; ++i)  // gradients in another order of dimensions are brought into the parameter's
+    if (!like(grads[i], params[i])) grads[i] = torch::empty_like(params[i]).copy_(grads[i]);
   auto stream = at::hip::getCurrentHIPStream();
   Args a;
   a.seed = static_cast<uint32_t>(seed);

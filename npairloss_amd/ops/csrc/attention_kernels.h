@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
   const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
   const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
   const int64_t bh = linear / q_tiles;
-  const int i0 = (q_tiles - 1 - static_cast<int>(linear % q_tiles)) * kQueries;
+  const int i0 = tile_at(linear % q_tiles, q_tiles, bh, a.causal && a.k_doc == nullptr) * kQueries;
   const int b = bh / a.H, h = bh % a.H, kv = h / (a.H / a.Hk);
   const int i = i0 + 32 * wave + lane % 32;
   const bool ok = i < a.Lq;
@@ -420,14 +420,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_spli
   uint32_t ids = 0;
   DocRange range{0, 0, 0}, range_next{0, 0, 0};
   uint64_t there = 0;
-  auto seek = [&](int j) {  // this wave's next tile of keys from j on
-    if (own != nullptr)
-      while (j < stop) {
-        range_next = own[j / kDocTile];
-        if (range_next.lo <= doc_hi && range_next.hi >= doc_lo) break;
-        j += KT * kWaves;
-      }
-    return j;
+  // This wave's next 32 keys: tiles of 64 that may hold ids of its rows go round by
+  // halves, two waves a tile.
+  TileWalk walk(own, doc_lo, doc_hi, split * keys_per_split / kDocTile, (stop + kDocTile - 1) / kDocTile);
+  int skip = wave / 2;
+  auto seek = [&]() {
+    for (; skip > 0; --skip)
+      if (walk.next() < 0) return stop;
+    skip = kWaves / 2 - 1;
+    const int n = walk.next();
+    if (n < 0) return stop;
+    if (own != nullptr) range_next = walk.of(n);
+    return min(n * kDocTile + wave % 2 * KT, stop);
   };
   using Way = Flight<T, DP, KT, 1>;
   auto load_k = [&](int j) {
@@ -441,7 +445,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_spli
   auto load_v = [&](int j) { Way::load(v0 + j * a.vs.l, a.vs.l, there, a.D, vs, 0); };
   // K of the next tile is asked for as soon as the scores have read this one's, V as
   // soon as the outputs have, so that half to all of a tile is always on its way.
-  int j = seek(split * keys_per_split + wave * KT);
+  int j = seek();
   if (j < stop) {
     load_k(j);
     load_v(j);
@@ -449,7 +453,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_spli
   while (j < stop) {
     if (own != nullptr && lane < KT) kd[wave][lane] = (there >> lane & 1) ? static_cast<int>(ids) : -1;
     range = range_next;
-    const int following = seek(j + KT * kWaves);
+    const int following = seek();
     Frag<T> p[1][2];
     f32x16 s[1];
     arrived<Way::kLoads>();  // K; V may still come
@@ -549,7 +553,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
   const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
   const int64_t bh = linear / q_tiles;
-  const int i0 = (q_tiles - 1 - static_cast<int>(linear % q_tiles)) * kQueries;
+  const int i0 = tile_at(linear % q_tiles, q_tiles, bh, a.causal && a.k_doc == nullptr) * kQueries;
   const int b = bh / a.H, h = bh % a.H, kv = h / (a.H / a.Hk);
   const int i = i0 + 32 * wave + lane % 32;
   const bool ok = i < a.Lq;
@@ -756,10 +760,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
   const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
   const int split = linear % splits;
   const int64_t bc = linear / splits / k_blocks;
-  // first, last, second, ..: a causal mask leaves the first blocks the most queries, and
-  // an XCD has a stretch of this order
+  // under a causal mask first, last, second, ..: the first blocks have the most queries,
+  // and an XCD has a stretch of this order
   const int place = static_cast<int>(linear / splits % k_blocks);
-  const int j0 = (place % 2 == 0 ? place / 2 : k_blocks - 1 - place / 2) * kKeys;
+  const int j0 = (!a.causal || a.k_doc != nullptr ? tile_at(place, k_blocks, bc, false) : place % 2 == 0 ? place / 2 : k_blocks - 1 - place / 2) * kKeys;
   const int b = bc / a.Hk, kv = bc % a.Hk, group = a.H / a.Hk, off = a.Lk - a.Lq;
   const int j = j0 + 32 * wave + lane % 32;
   const int doc = j < a.Lk && a.k_doc != nullptr ? a.k_doc[static_cast<int64_t>(b) * a.Lk + j] : 0;

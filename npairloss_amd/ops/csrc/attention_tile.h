@@ -198,6 +198,16 @@ DEVINL void arrived() {
 // All reads of shared memory of this wave are in registers.
 DEVINL void read_out() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// The tile of a head that place `i` of `n` takes.  Under a causal mask the last tiles
+// are the longest and go first.  Otherwise heads begin at different tiles: workgroups
+// that are a multiple of an XCD's CUs apart start on the same CU, and would all be
+// the same tile of several heads, all long or all short.
+DEVINL int tile_at(int i, int n, int64_t head, bool longest_first) {
+  if (longest_first) return n - 1 - i;
+  const uint32_t turn = static_cast<uint32_t>((static_cast<uint64_t>(static_cast<uint32_t>(head) * 0x9E3779B9u) * n) >> 32);
+  return (i + turn) % n;
+}
+
 // One word a thread, the first `n` of them, on the same way.
 DEVINL uint32_t staged_word(const void* base, int t, int n) {
   auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);

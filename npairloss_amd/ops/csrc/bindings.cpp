@@ -66,13 +66,14 @@ torch::Tensor gemm_tn(torch::Tensor A, torch::Tensor B);
 std::vector<torch::Tensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight,
                                         c10::optional<torch::Tensor> residual, double eps,
                                         int64_t group);
-std::vector<torch::Tensor> rms_norm_bwd(torch::Tensor dy, c10::optional<torch::Tensor> dsum,
-                                        torch::Tensor s, torch::Tensor weight, torch::Tensor inv);
 
-// rotary.hip
-std::vector<torch::Tensor> rotary_turn(torch::Tensor q, c10::optional<torch::Tensor> k,
-                                       torch::Tensor positions, torch::Tensor frequencies,
-                                       bool interleaved, double amplitude, bool backward);
+// autograd.cpp
+std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps);
+std::vector<torch::Tensor> rotary(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
+                                  torch::Tensor frequencies, bool interleaved, double amplitude);
+torch::Tensor attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double softcap,
+                        c10::optional<torch::Tensor> slopes, bool causal, c10::optional<torch::Tensor> prefix,
+                        c10::optional<torch::Tensor> q_doc, c10::optional<torch::Tensor> k_doc);
 
 // adamw.hip
 void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> grads,
@@ -80,17 +81,6 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
                   std::vector<torch::Tensor> steps, std::vector<torch::Tensor> masters,
                   std::vector<torch::Tensor> scales, double lr, double b1, double b2, double eps,
                   double weight_decay, int64_t seed);
-
-// attention.hip
-std::vector<torch::Tensor> attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double softcap,
-                                         c10::optional<torch::Tensor> slopes, bool causal,
-                                         c10::optional<torch::Tensor> prefix, c10::optional<torch::Tensor> q_doc,
-                                         c10::optional<torch::Tensor> k_doc, bool keep_rest);
-std::vector<torch::Tensor> attention_bwd(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
-                                         torch::Tensor o, torch::Tensor lse, torch::Tensor rest, double scale, double softcap,
-                                         c10::optional<torch::Tensor> slopes, bool causal,
-                                         c10::optional<torch::Tensor> prefix, c10::optional<torch::Tensor> q_doc,
-                                         c10::optional<torch::Tensor> k_doc);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "npairloss_amd gfx950 HIP kernels";
@@ -117,10 +107,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("conv1x1_dgrad", &conv1x1_dgrad, "1x1-conv data gradient GEMM (bf16 MFMA)");
   m.def("gemm_nn", &gemm_nn, "fp32 MFMA GEMM A @ B");
   m.def("rms_norm_fwd", &rms_norm_fwd, "residual + RMS norm, in the input's type or e4m3");
-  m.def("rms_norm_bwd", &rms_norm_bwd, "RMS norm gradients");
-  m.def("rotary_turn", &rotary_turn, "rotary positions for q and k");
+  m.def("rms_norm", &rms_norm, "residual + RMS norm, differentiable");
+  m.def("rotary", &rotary, "rotary positions for q and k, differentiable");
+  m.def("attention", &attention, "masked attention, differentiable");
   m.def("adamw_update", &adamw_update, "AdamW step over many tensors, fp32 or 8-bit moments");
-  m.def("attention_fwd", &attention_fwd, "masked attention forward");
-  m.def("attention_bwd", &attention_bwd, "masked attention gradients");
   m.def("gemm_tn", &gemm_tn, "fp32 MFMA GEMM A^T @ B");
 }

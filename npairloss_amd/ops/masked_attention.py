@@ -104,48 +104,29 @@ def _backward_torch(g, q, k, v, o, lse, scale, softcap, slopes, causal, prefix, 
 # autograd binding
 # ---------------------------------------------------------------------------
 
-def _ready(x, width):
-    """Rows as the kernels read them: `width` wide (zeros behind), 16-byte borders."""
-    if x.shape[-1] != width:
-        return torch.nn.functional.pad(x, (0, width - x.shape[-1]))
-    per16 = 16 // x.element_size()
-    far = x.shape[1] > 1 and x.stride(1) * x.element_size() > 1 << 24  # offsets within a tile are 32 bits
-    if x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % per16 for s in x.stride()[:3]) or far:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
 class _AttentionFn(torch.autograd.Function):
+    """On the CPU, and where there is nothing to attend to; GPU tensors are recorded in
+    csrc/autograd.cpp."""
+
     @staticmethod
-    def forward(ctx, q, k, v, scale, softcap, slopes, causal, prefix, q_doc, k_doc, train):
-        how = (scale, softcap, slopes, causal, prefix, q_doc, k_doc)
-        ctx.how, ctx.width = (scale, softcap, causal), q.shape[-1]
+    def forward(ctx, q, k, v, scale, softcap, slopes, causal, prefix, q_doc, k_doc):
+        ctx.how = (scale, softcap, causal)
         ctx.empty = q.numel() == 0 or k.numel() == 0
         if ctx.empty:
             ctx.save_for_backward(q, k, v)
             return torch.zeros_like(q, memory_format=torch.contiguous_format)
-        if q.is_cuda:
-            width = -(-ctx.width // 8) * 8
-            q, k, v = (_ready(x, width) for x in (q, k, v))
-            o, lse, rest = _backend.ext().attention_fwd(q, k, v, *how, train)
-        else:
-            (o, lse), rest = _forward_torch(q, k, v, *how), None
-        ctx.save_for_backward(q, k, v, o, lse, rest, slopes, prefix, q_doc, k_doc)
-        return o[..., :ctx.width]
+        o, lse = _forward_torch(q, k, v, scale, softcap, slopes, causal, prefix, q_doc, k_doc)
+        ctx.save_for_backward(q, k, v, o, lse, slopes, prefix, q_doc, k_doc)
+        return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         if ctx.empty:
-            return tuple(torch.zeros_like(x) for x in ctx.saved_tensors) + (None,) * 8
-        q, k, v, o, lse, rest, slopes, prefix, q_doc, k_doc = ctx.saved_tensors
+            return tuple(torch.zeros_like(x) for x in ctx.saved_tensors) + (None,) * 7
+        q, k, v, o, lse, slopes, prefix, q_doc, k_doc = ctx.saved_tensors
         scale, softcap, causal = ctx.how
-        how = (scale, softcap, slopes, causal, prefix, q_doc, k_doc)
-        if q.is_cuda:
-            grads = _backend.ext().attention_bwd(_ready(g, q.shape[-1]), q, k, v, o, lse, rest, *how)
-        else:
-            grads = _backward_torch(g, q, k, v, o, lse, *how)
-        return tuple(x[..., :ctx.width] for x in grads) + (None,) * 8
+        return tuple(_backward_torch(g, q, k, v, o, lse, scale, softcap, slopes, causal, prefix, q_doc, k_doc)) + (None,) * 7
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, softcap: float = 0.0,
@@ -200,5 +181,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
             raise ValueError(f"attention: tensors on {q.device} and {x.device}")
     slopes, prefix, documents, key_documents = (x if x is None else x.detach().contiguous()
                                                 for x in (slopes, prefix, documents, key_documents))
-    train = torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v))
-    return _AttentionFn.apply(q, k, v, scale, float(softcap), slopes, bool(causal), prefix, documents, key_documents, train)
+    args = (q, k, v, scale, float(softcap), slopes, bool(causal), prefix, documents, key_documents)
+    if q.is_cuda and q.numel() and k.numel():
+        return _backend.ext().attention(*args)
+    return _AttentionFn.apply(*args)

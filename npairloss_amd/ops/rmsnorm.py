@@ -48,20 +48,15 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 
 class _RMSNormFn(torch.autograd.Function):
+    """On the CPU; GPU tensors are recorded in csrc/autograd.cpp."""
+
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        ctx.gpu = x.is_cuda
         ctx.has_residual = residual is not None
-        weight = weight.contiguous()
-        if x.is_cuda:
-            got = _backend.ext().rms_norm_fwd(_rows(x), weight, None if residual is None else _rows(residual), eps, -1)
-            y, inv = got[0].view(x.shape), got[1]
-            s = got[2].view(x.shape) if ctx.has_residual else x
-        else:
-            s = x + residual if ctx.has_residual else x
-            sf = s.float().contiguous()
-            inv = torch.rsqrt(sf.square().mean(-1) + eps)
-            y = (sf * inv.unsqueeze(-1) * weight.float()).to(x.dtype)
+        s = x + residual if ctx.has_residual else x
+        sf = s.float().contiguous()
+        inv = torch.rsqrt(sf.square().mean(-1) + eps)
+        y = (sf * inv.unsqueeze(-1) * weight.float()).to(x.dtype)
         ctx.save_for_backward(s, weight, inv)
         ctx.set_materialize_grads(False)
         return (y, s) if ctx.has_residual else y
@@ -72,15 +67,11 @@ class _RMSNormFn(torch.autograd.Function):
         s, weight, inv = ctx.saved_tensors
         if dy is None:  # only the sum was used
             return dsum, None, dsum, None
-        if ctx.gpu:
-            dx, dw = _backend.ext().rms_norm_bwd(_rows(dy), None if dsum is None else _rows(dsum), _rows(s), weight, inv)
-            dx = dx.view(s.shape)
-        else:
-            n, g = s.float() * inv.unsqueeze(-1), dy.float()
-            dw = (g * n).reshape(-1, n.shape[-1]).sum(0).to(weight.dtype)
-            g = g * weight.float()
-            dx = inv.unsqueeze(-1) * (g - n * (g * n).mean(-1, keepdim=True))
-            dx = (dx if dsum is None else dx + dsum.float()).to(s.dtype)
+        n, g = s.float() * inv.unsqueeze(-1), dy.float()
+        dw = (g * n).reshape(-1, n.shape[-1]).sum(0).to(weight.dtype)
+        g = g * weight.float()
+        dx = inv.unsqueeze(-1) * (g - n * (g * n).mean(-1, keepdim=True))
+        dx = (dx if dsum is None else dx + dsum.float()).to(s.dtype)
         return dx, dw, dx if ctx.has_residual else None, None
 
 
@@ -89,6 +80,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     """y, or with a residual (y, s), s = x + residual rounded to x's type; both
     differentiable.  `weight` is of x's type or fp32."""
     _check(x, weight, residual)
+    if x.is_cuda:
+        out = _backend.ext().rms_norm(x, weight, residual, float(eps))
+        return out[0] if residual is None else (out[0], out[1])
     return _RMSNormFn.apply(x, weight, residual, float(eps))
 
 

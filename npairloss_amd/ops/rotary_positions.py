@@ -75,15 +75,14 @@ def _turn_torch(x, angle, interleaved, amplitude, backward):
 
 
 def _turn(q, k, positions, frequencies, interleaved, amplitude, backward):
-    if q.is_cuda:
-        q, k = (x if x is None or x.stride(-1) == 1 else x.contiguous() for x in (q, k))
-        return _backend.ext().rotary_turn(q, k, positions, frequencies.reshape(-1), interleaved, amplitude, backward)
     f = frequencies.reshape(positions.shape[-1], -1)
     angle = (positions.double().unsqueeze(-1) * f).flatten(-2)
     return [_turn_torch(x, angle, interleaved, amplitude, backward) for x in (q, k) if x is not None]
 
 
 class _RotaryFn(torch.autograd.Function):
+    """On the CPU; GPU tensors are recorded in csrc/autograd.cpp."""
+
     @staticmethod
     def forward(ctx, q, k, positions, frequencies, interleaved, amplitude):
         ctx.save_for_backward(positions, frequencies)
@@ -135,4 +134,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         if t is not None and t.device != q.device:
             raise ValueError(f"rotary: tensors on {q.device} and {t.device}")
     positions = positions.reshape(*lead, *axes).expand(q.shape[0], q.shape[1], *axes)
-    return _RotaryFn.apply(q, k, positions, frequencies.contiguous(), bool(interleaved), float(amplitude))
+    if q.is_cuda:
+        out = _backend.ext().rotary(q, k, positions, frequencies.reshape(-1), bool(interleaved), float(amplitude))
+        return out[0] if k is None else (out[0], out[1])
+    return _RotaryFn.apply(q, k, positions, frequencies, bool(interleaved), float(amplitude))

@@ -26,6 +26,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = [
     "bindings.cpp",
+    "autograd.cpp",
     "npair_rows.hip",
     "sort_select.hip",
     "l2norm.hip",
