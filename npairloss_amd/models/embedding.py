@@ -10,7 +10,7 @@ from torch import nn
 from ..ops.l2norm import l2_normalize
 from .googlenet import GoogLeNet
 from .resnet import ResNet50
-from .vit import ViTB16
+from .vit import RotaryViTB16, ViTB16
 
 
 class EmbeddingNet(nn.Module):
@@ -21,7 +21,13 @@ class EmbeddingNet(nn.Module):
         self.embed_dim = getattr(backbone, "embed_dim", None)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        f = self.backbone(x)
+        return self._embedded(self.backbone(x))
+
+    def forward_packed(self, images, row_length: int = 0) -> torch.Tensor:
+        """Embeddings of images of any sizes, where the backbone packs them."""
+        return self._embedded(self.backbone.forward_packed(images, row_length))
+
+    def _embedded(self, f: torch.Tensor) -> torch.Tensor:
         if f.dim() != 2:
             f = f.flatten(1)
         if self.normalize:
@@ -42,6 +48,8 @@ def build_embedding_model(name: str, embed_dim: int = None, normalize: bool = Tr
         bb = ResNet50(embed_dim=embed_dim or 128)
     elif name in ("vit", "vit-b/16", "vitb16"):
         bb = ViTB16(embed_dim=embed_dim or 768)
+    elif name in ("vit-rotary", "vit_rotary"):
+        bb = RotaryViTB16(embed_dim=embed_dim or 768)
     else:
         raise ValueError(f"unknown backbone {name!r}")
     return EmbeddingNet(bb, normalize=normalize)

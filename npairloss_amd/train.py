@@ -27,7 +27,7 @@ def main(argv=None):
                    help="bf16 model + fp32 master weights (replaces --amp)")
     p.add_argument("--num-workers", type=int, default=2)
     p.add_argument("--backbone", default=None,
-                   help="override the backbone (googlenet/resnet50/vit)")
+                   help="override the backbone (googlenet/resnet50/vit/vit-rotary)")
     p.add_argument("--graph", dest="graph", action="store_true", default=None,
                    help="hipGraph whole-step capture+replay (default ON on "
                         "GPU; the bench's headline mode — lazy capture after "
