@@ -1,6 +1,6 @@
-// The transformer operators as differentiable calls on GPU tensors.  Recorded here
-// and not in Python: a pass over a few MB takes the GPU some 15 us, and a Python
-// function forward and backward twice that and more.
+// The transformer operators as differentiable calls on GPU tensors.  Checked and
+// recorded here and not in Python: a pass over a few MB takes the GPU some 15 us, one
+// over a token 3, and a Python function forward and backward takes 40 and more.
 
 #include <torch/extension.h>
 
@@ -35,14 +35,37 @@ void once(const char* name) {  // under create_graph=True the engine records wha
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its gradient has no gradient");
 }
 
-Tensor rows(const Tensor& x) { return x.reshape({-1, x.size(-1)}).contiguous(); }
+Tensor rows(const Tensor& x) {
+  if (x.dim() == 2 && x.is_contiguous()) return x;
+  return x.reshape({x.size(-1) > 0 ? x.numel() / x.size(-1) : 0, x.size(-1)}).contiguous();
+}
+
+Tensor shaped(const Tensor& x, at::IntArrayRef sizes) { return x.sizes() == sizes ? x : x.view(sizes); }
+
+bool floating(const Tensor& x) {
+  return x.scalar_type() == at::kFloat || x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf;
+}
+
+void check_norm(const Tensor& x, const Tensor& weight, const OptTensor& residual) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "rms_norm: 1 to 16384 columns expected, got shape ", x.sizes());
+  TORCH_CHECK_TYPE(floating(x), "rms_norm: fp32, bf16 or fp16 expected, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == x.size(-1), "rms_norm: weight ", weight.sizes(), " does not fit rows of ", x.size(-1));
+  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, "rms_norm: weight is ",
+                   weight.scalar_type(), ", x is ", x.scalar_type());
+  TORCH_CHECK_VALUE(weight.device() == x.device(), "rms_norm: tensors on ", x.device(), " and ", weight.device());
+  if (residual.has_value()) {
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(), "rms_norm: residual ", residual->sizes(),
+                      " ", residual->scalar_type(), " does not match x ", x.sizes(), " ", x.scalar_type());
+    TORCH_CHECK_VALUE(residual->device() == x.device(), "rms_norm: tensors on ", x.device(), " and ", residual->device());
+  }
+}
 
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps) {
     const Tensor w = weight.contiguous();
     auto got = rms_norm_fwd(rows(x), w, residual.has_value() ? OptTensor(rows(*residual)) : c10::nullopt, eps, -1);
-    variable_list out{got[0].view(x.sizes())};
-    if (residual.has_value()) out.push_back(got[2].view(x.sizes()));
+    variable_list out{shaped(got[0], x.sizes())};
+    if (residual.has_value()) out.push_back(shaped(got[2], x.sizes()));
     ctx->save_for_backward({residual.has_value() ? out[1] : x, w, got[1]});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->set_materialize_grads(false);
@@ -56,7 +79,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const Tensor dsum = residual ? grads[1] : Tensor();
     if (!grads[0].defined()) return {dsum, Tensor(), dsum, Tensor()};  // only the sum was used
     auto got = rms_norm_bwd(rows(grads[0]), dsum.defined() ? OptTensor(rows(dsum)) : c10::nullopt, rows(saved[0]), saved[1], saved[2]);
-    const Tensor dx = got[0].view(saved[0].sizes());
+    const Tensor dx = shaped(got[0], saved[0].sizes());
     return {dx, got[1], residual ? dx : Tensor(), Tensor()};
   }
 };
@@ -134,11 +157,58 @@ struct Attention : torch::autograd::Function<Attention> {
 }  // namespace
 
 std::vector<Tensor> rms_norm(Tensor x, Tensor weight, OptTensor residual, double eps) {
+  check_norm(x, weight, residual);
   return RmsNorm::apply(x, weight, residual, eps);
 }
 
+// {codes, scales} and the sum, if there is a residual.
+std::vector<Tensor> rms_norm_fp8(Tensor x, Tensor weight, OptTensor residual, double eps, int64_t group) {
+  check_norm(x, weight, residual);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad() || (residual.has_value() && residual->requires_grad())),
+              "rms_norm_fp8 has no gradient: call it under torch.no_grad()");
+  const int64_t D = x.size(-1);
+  TORCH_CHECK_VALUE(group == 0 || (group >= 16 && group <= 512 && (group & (group - 1)) == 0 && D % group == 0), "rms_norm_fp8: group ", group,
+                    " is not a power of two from 16 to 512 that divides ", D);
+  // groups want eight neighbours to a lane: rows that begin off a 16-byte border are copied
+  auto placed = [&](const Tensor& t) { return group > 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0 ? t.clone() : t; };
+  auto got = rms_norm_fwd(placed(rows(x)), placed(weight.contiguous()), residual.has_value() ? OptTensor(placed(rows(*residual))) : c10::nullopt,
+                          eps, group);
+  if (x.dim() != 2) {
+    auto sizes = x.sizes().vec();
+    got[0] = got[0].view(sizes);
+    if (residual.has_value()) got[2] = got[2].view(sizes);
+    sizes.back() = got[1].size(1);
+    got[1] = got[1].view(sizes);
+  }
+  return got;
+}
+
 std::vector<Tensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor frequencies, bool interleaved, double amplitude) {
-  return Rotary::apply(q, k, positions, frequencies, interleaved, amplitude);
+  auto check = [&](const Tensor& x, const char* name) {
+    TORCH_CHECK_VALUE(x.dim() == 4, "rotary: ", name, " is [batch, length, heads, width], got ", x.sizes());
+    TORCH_CHECK_TYPE(floating(x) && x.scalar_type() == q.scalar_type(), "rotary: q and k are fp32, bf16 or fp16 of one type, got ", name, " ",
+                     x.scalar_type());
+    TORCH_CHECK_VALUE(x.size(0) == q.size(0) && x.size(1) == q.size(1) && x.size(3) == q.size(3), "rotary: q ", q.sizes(), " and k ", x.sizes(),
+                      " do not go together");
+  };
+  check(q, "q");
+  if (k.has_value()) check(*k, "k");
+  TORCH_CHECK_TYPE(frequencies.scalar_type() == at::kDouble && (frequencies.dim() == 1 || frequencies.dim() == 2),
+                   "rotary: frequencies are fp64 [n] or [axes, n], got ", frequencies.scalar_type(), " ", frequencies.sizes());
+  const int64_t P = frequencies.numel();
+  TORCH_CHECK_VALUE(P >= 1 && P <= 512 && 2 * P <= q.size(3), "rotary: ", P, " frequencies do not fit heads of ", q.size(3), " (at most 512)");
+  TORCH_CHECK_TYPE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "rotary: positions are int32 or int64, got ",
+                   positions.scalar_type());
+  const bool axes = frequencies.dim() == 2;
+  const int64_t lead = positions.dim() - axes;
+  TORCH_CHECK_VALUE((lead == 1 || lead == 2) && positions.size(lead - 1) == q.size(1) && (lead == 1 || positions.size(0) == q.size(0)) &&
+                        (!axes || positions.size(lead) == frequencies.size(0)),
+                    "rotary: positions ", positions.sizes(), " do not fit q ", q.sizes(), " and frequencies ", frequencies.sizes());
+  for (const Tensor& x : {k.value_or(q), positions, frequencies})
+    TORCH_CHECK_VALUE(x.device() == q.device(), "rotary: tensors on ", q.device(), " and ", x.device());
+  if (!axes) positions = positions.unsqueeze(-1);
+  if (lead == 1) positions = positions.unsqueeze(0).expand({q.size(0), q.size(1), positions.size(-1)});
+  return Rotary::apply(q, k, positions, frequencies.is_contiguous() ? frequencies : frequencies.contiguous(), interleaved, amplitude);
 }
 
 Tensor attention(Tensor q, Tensor k, Tensor v, double scale, double softcap, OptTensor slopes, bool causal, OptTensor prefix,

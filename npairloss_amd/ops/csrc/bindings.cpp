@@ -62,13 +62,10 @@ torch::Tensor sim_gemm_nt(torch::Tensor F_l, torch::Tensor F_g);
 torch::Tensor gemm_nn(torch::Tensor A, torch::Tensor B);
 torch::Tensor gemm_tn(torch::Tensor A, torch::Tensor B);
 
-// rms_norm.hip
-std::vector<torch::Tensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight,
-                                        c10::optional<torch::Tensor> residual, double eps,
-                                        int64_t group);
-
 // autograd.cpp
 std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps);
+std::vector<torch::Tensor> rms_norm_fp8(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual, double eps,
+                                        int64_t group);
 std::vector<torch::Tensor> rotary(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
                                   torch::Tensor frequencies, bool interleaved, double amplitude);
 torch::Tensor attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double softcap,
@@ -106,8 +103,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused 1x1-conv GEMM + bias + relu (bf16 MFMA)");
   m.def("conv1x1_dgrad", &conv1x1_dgrad, "1x1-conv data gradient GEMM (bf16 MFMA)");
   m.def("gemm_nn", &gemm_nn, "fp32 MFMA GEMM A @ B");
-  m.def("rms_norm_fwd", &rms_norm_fwd, "residual + RMS norm, in the input's type or e4m3");
   m.def("rms_norm", &rms_norm, "residual + RMS norm, differentiable");
+  m.def("rms_norm_fp8", &rms_norm_fp8, "residual + RMS norm, in e4m3 with scales");
   m.def("rotary", &rotary, "rotary positions for q and k, differentiable");
   m.def("attention", &attention, "masked attention, differentiable");
   m.def("adamw_update", &adamw_update, "AdamW step over many tensors, fp32 or 8-bit moments");

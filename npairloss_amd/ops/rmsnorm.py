@@ -43,10 +43,6 @@ def _check(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tenso
             raise ValueError(f"rms_norm: tensors on {x.device} and {t.device}")
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    return x.reshape(-1, x.shape[-1]).contiguous()
-
-
 class _RMSNormFn(torch.autograd.Function):
     """On the CPU; GPU tensors are recorded in csrc/autograd.cpp."""
 
@@ -79,10 +75,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
              eps: float = 1e-6) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """y, or with a residual (y, s), s = x + residual rounded to x's type; both
     differentiable.  `weight` is of x's type or fp32."""
+    if x.is_cuda:  # checked there, as below
+        out = _backend.ext().rms_norm(x, weight, residual, eps)
+        return out[0] if residual is None else tuple(out)
     _check(x, weight, residual)
-    if x.is_cuda:
-        out = _backend.ext().rms_norm(x, weight, residual, float(eps))
-        return out[0] if residual is None else (out[0], out[1])
     return _RMSNormFn.apply(x, weight, residual, float(eps))
 
 
@@ -94,21 +90,14 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     magnitude it covers over 448.  `group` is a power of two from 16 to 512 that
     divides D.  A row that holds NaN gets NaN codes and scales.  No gradient:
     inputs that require one are refused while gradients are recorded."""
+    if x.is_cuda:  # checked there, as below
+        return tuple(_backend.ext().rms_norm_fp8(x, weight, residual, eps, group))
     _check(x, weight, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
-    D = x.shape[-1]
+    D, lead = x.shape[-1], x.shape[:-1]
     if group != 0 and (group < 16 or group > 512 or group & (group - 1) or D % group):
         raise ValueError(f"rms_norm_fp8: group {group} is not a power of two from 16 to 512 that divides {D}")
-    lead = x.shape[:-1]
-    if x.is_cuda:
-        x2, w = _rows(x), weight.contiguous()
-        r2 = None if residual is None else _rows(residual)
-        if group:  # eight neighbours to a lane: rows that begin off a 16-byte border are copied
-            x2, w, r2 = (t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in (x2, w, r2))
-        got = _backend.ext().rms_norm_fwd(x2, w, r2, float(eps), int(group))
-        codes, scales = got[0].view(x.shape), got[1].view(*lead, got[1].shape[1])
-        return (codes, scales) if residual is None else (codes, scales, got[2].view(x.shape))
     s = x if residual is None else x + residual
     sf = s.float().contiguous()
     y = sf * torch.rsqrt(sf.square().mean(-1, keepdim=True) + eps) * weight.float()

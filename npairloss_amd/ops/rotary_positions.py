@@ -109,6 +109,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     [batch, length], with one more dimension of axes where `frequencies` is
     [axes, n] (axis a turns pairs a n to a n + n).  `frequencies` is fp64, from
     `rotary_frequencies`; cosines and sines are multiplied by `amplitude`."""
+    if q.is_cuda:  # checked there, as below
+        out = _backend.ext().rotary(q, k, positions, frequencies, interleaved, amplitude)
+        return out[0] if k is None else tuple(out)
     for name, x in (("q", q), ("k", k)):
         if x is None:
             continue
@@ -134,7 +137,4 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         if t is not None and t.device != q.device:
             raise ValueError(f"rotary: tensors on {q.device} and {t.device}")
     positions = positions.reshape(*lead, *axes).expand(q.shape[0], q.shape[1], *axes)
-    if q.is_cuda:
-        out = _backend.ext().rotary(q, k, positions, frequencies.reshape(-1), bool(interleaved), float(amplitude))
-        return out[0] if k is None else (out[0], out[1])
     return _RotaryFn.apply(q, k, positions, frequencies, bool(interleaved), float(amplitude))
