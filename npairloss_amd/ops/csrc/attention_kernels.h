@@ -44,7 +44,8 @@ struct ScoreMap {
 
   // `apart`: what the lane's index is ahead of the first register's of half 0.
   DEVINL ScoreMap(const AttnArgs& a, float slope, int apart) {
-    const float c = fabsf(a.scale) * kLog2e;
+    // not 0: what is not seen is -infinity here, and 0 times that is not a number
+    const float c = fmaxf(fabsf(a.scale) * kLog2e, FLT_MIN);
     factor = SC == kPlain ? c : 1.f;
     in = capped(SC) ? fabsf(a.scale) / a.softcap : c;
     out = a.softcap * kLog2e;
@@ -68,22 +69,39 @@ struct ScoreMap {
   }
 };
 
-// Which registers a query sees, as bits.
-DEVINL uint32_t seen_keys(const AttnArgs& a, const Query& q, const int* kd, int first, int row0) {
-  const int half = threadIdx.x % WAVE / 32, left = q.end - first - 4 * half;
-  uint32_t seen = 0;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) seen |= static_cast<uint32_t>(result_row(r, 0) < left) << r;
-  if (a.k_doc != nullptr) {
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int4 d = *reinterpret_cast<const int4*>(kd + row0 + 8 * x + 4 * half);
-      const uint32_t same = static_cast<uint32_t>(d.x == q.doc) | static_cast<uint32_t>(d.y == q.doc) << 1 |
-                            static_cast<uint32_t>(d.z == q.doc) << 2 | static_cast<uint32_t>(d.w == q.doc) << 3;
-      seen &= same << (4 * x) | ~(15u << (4 * x));
-    }
+// What a tile's masks ask of every pair: no question, an end (or a beginning), an id as
+// well.
+enum Mask { kSeen, kEnds, kIds };
+
+// Which of the pairs (lane, register) are seen.  `left`: registers' rows before it,
+// from half 0 on; with FROM, rows from it on.  `ids`: of the registers' rows; `doc`: the
+// lane's, one that no row has if it is negative.
+template <Mask MASK, bool FROM>
+struct Seen {
+  int bound, doc;
+  const int* ids;
+  int4 four;
+
+  DEVINL Seen(int bound_, int doc_, const int* ids_) {
+    const int half = threadIdx.x % WAVE / 32;
+    bound = bound_ - 4 * half;
+    doc = doc_ < 0 ? -2 : doc_;
+    ids = ids_ + 4 * half;
   }
-  return seen;
+
+  DEVINL bool operator()(int r) {
+    bool ok = FROM ? result_row(r, 0) >= bound : result_row(r, 0) < bound;
+    if (MASK == kIds) {
+      if (r % 4 == 0) four = *reinterpret_cast<const int4*>(ids + 2 * r);
+      ok = ok && (r % 4 == 0 ? four.x : r % 4 == 1 ? four.y : r % 4 == 2 ? four.z : four.w) == doc;
+    }
+    return ok;
+  }
+};
+
+// x, or 0 where bit r is not set.
+DEVINL float with_bit(float x, uint32_t bits, int r) {
+  return __uint_as_float(__float_as_uint(x) & static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - r)) >> 31));
 }
 
 // --- forward ----------------------------------------------------------------
@@ -104,14 +122,14 @@ struct Online {
     l = 0.f;
   }
 
-  template <Score SC, bool MASKED>
+  template <Score SC>
   DEVINL void absorb(const AttnArgs& a, const Reader<T, DP>& reader, const Frag<T> (&qf)[DP / 16], const T* ks, const T* vs, const int* kd,
-                     const Query& q, int first) {
+                     const Query& q, int first, Mask mask) {
     const Reader<T, DP> at = reader.fresh();
     Frag<T> p[NS][2];
     f32x16 s[NS];
     scores(at, qf, ks, s);
-    weights<SC, MASKED>(a, s, p, kd, q, first);
+    weights<SC>(a, s, p, kd, q, first, mask);
     outputs(at, vs, p);
   }
 
@@ -123,23 +141,33 @@ struct Online {
                              [&](auto i, const Frag<T>& k) { product(k, qf[i % kSteps], s[i / kSteps]); });
   }
 
-  template <Score SC, bool MASKED>
-  DEVINL void weights(const AttnArgs& a, f32x16 (&s)[NS], Frag<T> (&p)[NS][2], const int* kd, const Query& q, int first) {
+  template <Score SC>
+  DEVINL void weights(const AttnArgs& a, f32x16 (&s)[NS], Frag<T> (&p)[NS][2], const int* kd, const Query& q, int first, Mask mask) {
     float c = 1.f, high = -INFINITY;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       const ScoreMap<T, SC> map(a, q.slope2, q.at - first - 32 * n);
       c = map.factor;
-      uint32_t seen = 0xFFFF;
-      if (MASKED) seen = seen_keys(a, q, kd, first + 32 * n, 32 * n);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float bend;
         s[n][r] = map(s[n][r], r, bend);
-        if (MASKED) s[n][r] = (seen >> r & 1) ? s[n][r] : -INFINITY;
-        high = fmaxf(high, s[n][r]);
       }
     }
+    auto apply = [&](auto which) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        Seen<decltype(which)::value, false> seen(q.end - first - 32 * n, q.doc, kd + 32 * n);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = seen(r) ? s[n][r] : -INFINITY;
+      }
+    };
+    if (mask == kEnds) apply(std::integral_constant<Mask, kEnds>());
+    if (mask == kIds) apply(std::integral_constant<Mask, kIds>());
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) high = fmaxf(high, s[n][r]);
     high = fmaxf(high, other_half(high)) * c;
     const float now = fmaxf(top, high), from = now == -INFINITY ? 0.f : now;
     const float keep = __builtin_amdgcn_exp2f(top - from);
@@ -226,7 +254,7 @@ DEVINL uint32_t bad_columns(bool bad) {
 // the sum; an fp16 operand may overflow.  Without masks and in types of fp32's
 // range the value is the formula's own.
 template <typename T>
-DEVINL bool repairs(const AttnArgs& a) { return sizeof(T) == 2 || a.causal || a.k_doc != nullptr; }
+DEVINL bool repairs(const AttnArgs& a) { return std::is_same<T, fp16_t>::value || a.causal || a.k_doc != nullptr; }
 
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void forward_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
@@ -317,8 +345,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
     if (j < most_end) {
       bool masked = j + KT > least_end;
       if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
-      if (masked) run.template absorb<SC, true>(a, at, qf, ks[kBuf], vs[kBuf], kd[kBuf], q, j);
-      else run.template absorb<SC, false>(a, at, qf, ks[kBuf], vs[kBuf], kd[kBuf], q, j);
+      run.template absorb<SC>(a, at, qf, ks[kBuf], vs[kBuf], kd[kBuf], q, j, !masked ? kSeen : own == nullptr ? kEnds : kIds);
     }
     landed(std::integral_constant<int, 1 - kBuf>());
     j = following;
@@ -462,8 +489,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_spli
     if (following < stop) load_k(following);
     bool masked = j + KT > least_end;
     if (own != nullptr) masked = masked || !(range.one() && doc_lo == doc_hi && range.lo == doc_lo);
-    if (masked) run.template weights<SC, true>(a, s, p, kd[wave], q, j);
-    else run.template weights<SC, false>(a, s, p, kd[wave], q, j);
+    run.template weights<SC>(a, s, p, kd[wave], q, j, !masked ? kSeen : own == nullptr ? kEnds : kIds);
     if (following < stop) arrived<Way::kLoads>();
     else arrived<0>();
     run.outputs(at, vs, p);
@@ -637,7 +663,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   // before, and those' products under the weights of these; with one, the other wave
   // of the SIMD has to fill the time.
   constexpr int kSub = KT / 32, kSteps = DP / 16, kWide = DP / 32;
-  auto step = [&](auto masked, int j, auto buf) {
+  auto step = [&](bool masked, int j, auto buf) {
     const Reader<T, DP> at = reader.fresh();
     f32x16 s[kSub], dp[kSub];
     Frag<T> ds[kSub][2];
@@ -649,43 +675,57 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
     auto score_read = [&](int n, int i) { return at.rows(i % 2 == 0 ? ks[buf] : vs[buf], 32 * n, i / 2); };
     auto output = [&](int n, int i, const Frag<T>& f) { product(f, ds[n][i / kWide], dq[i % kWide]); };
     auto output_read = [&](int n, int i) { return at.columns(ks[buf], 32 * n + 16 * (i / kWide), i % kWide); };
-    uint32_t seen[kSub];
-    auto weight = [&](int n, int r) {  // registers r and r + 1
+    uint32_t bits[kSub];  // one body for all tiles, as for dK and dV
+    auto mask = [&](int n) {
+      bits[n] = ~0u;
+      auto apply = [&](auto which) {
+        Seen<decltype(which)::value, false> seen(q.end - j - 32 * n, q.doc, kd[buf] + 32 * n);
+        if (capped(SC)) bits[n] = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (capped(SC)) bits[n] |= static_cast<uint32_t>(seen(r)) << r;
+          else s[n][r] = seen(r) ? s[n][r] : -INFINITY;
+        }
+      };
+      if (masked && own == nullptr) apply(std::integral_constant<Mask, kEnds>());
+      if (masked && own != nullptr) apply(std::integral_constant<Mask, kIds>());
+    };
+    auto weight = [&](int n, int r) {  // registers r and r + 1, in their order
       const ScoreMap<T, SC> map(a, q.slope2, q.at - j - 32 * n);
-      if (masked && r == 0) seen[n] = seen_keys(a, q, kd[buf], j + 32 * n, 32 * n);
       float x[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         float bend;
         const float t = map(s[n][r + y], r + y, bend);
-        x[y] = __builtin_amdgcn_exp2f(fmaf(t, map.factor, -lse)) * (dp[n][r + y] - delta);
+        x[y] = __builtin_amdgcn_exp2f(fmaf(t, map.factor, -lse));
+        if (capped(SC)) x[y] = with_bit(x[y], bits[n], r + y);
+        x[y] *= dp[n][r + y] - delta;
         if (capped(SC)) x[y] *= bend;
-        if (masked) x[y] = (seen[n] >> (r + y) & 1) ? x[y] : 0.f;
       }
       ds[n][r / 8].set2(r % 8, x[0], x[1]);
     };
     constexpr int kA = 2 * kSteps, kB = 2 * kWide;  // products of scores and of outputs
     if constexpr (kSub == 2 && DP == 64) {
-      piped<T, 2 * kA + 2 * kB, 4>(
-          [&](auto i) { return i < 2 * kA ? score_read(i / kA, i % kA) : output_read((i - 2 * kA) / kB, (i - 2 * kA) % kB); },
-          [&](auto i, const Frag<T>& f) {
-            if (i < kA) {
-              score(0, i, f);
-            } else if (i < 2 * kA) {
-              score(1, i - kA, f);
+      piped<T, kA, 4>([&](auto i) { return score_read(0, i); }, [&](auto i, const Frag<T>& f) { score(0, i, f); });
+      mask(0);
+      piped<T, kA, 4>([&](auto i) { return score_read(1, i); },
+                      [&](auto i, const Frag<T>& f) {
+                        score(1, i, f);
 #pragma unroll
-              for (int r = 16 / kA * (i - kA); r < 16 / kA * (i - kA + 1); r += 2) weight(0, r);
-            } else if (i < 2 * kA + kB) {
-              output(0, i - 2 * kA, f);
+                        for (int r = 16 / kA * i; r < 16 / kA * (i + 1); r += 2) weight(0, r);
+                      });
+      mask(1);
+      piped<T, 2 * kB, 4>([&](auto i) { return output_read(i / kB, i % kB); },
+                          [&](auto i, const Frag<T>& f) {
+                            output(i / kB, i % kB, f);
+                            if (i < kB)
 #pragma unroll
-              for (int r = 16 / kB * (i - 2 * kA); r < 16 / kB * (i - 2 * kA + 1); r += 2) weight(1, r);
-            } else {
-              output(1, i - 2 * kA - kB, f);
-            }
-          });
+                              for (int r = 16 / kB * i; r < 16 / kB * (i + 1); r += 2) weight(1, r);
+                          });
     } else {
       each(std::make_integer_sequence<int, kSub>(), [&](auto n) {
         piped<T, kA, 4>([&](auto i) { return score_read(n, i); }, [&](auto i, const Frag<T>& f) { score(n, i, f); });
+        mask(n);
 #pragma unroll
         for (int r = 0; r < 16; r += 2) weight(n, r);
         __builtin_amdgcn_sched_barrier(0);
@@ -722,8 +762,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
     if (j < most_end) {
       bool masked = j + KT > least_end;
       if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
-      if (masked) step(std::true_type(), j, buf);
-      else step(std::false_type(), j, buf);
+      step(masked, j, buf);
     }
     landed(std::integral_constant<int, 1 - kBuf>());
     j = following;
@@ -839,7 +878,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
   // The scores of 32 queries pass under the weights of the 32 before, and those'
   // products under the weights of these.
   constexpr int kSub = QT / 32, kSteps = DP / 16, kWide = DP / 32;
-  auto step = [&](auto masked, int i0, float slope2, auto buf) {
+  auto step = [&](bool masked, int i0, float slope2, auto buf) {
     const Reader<T, DP> at = reader.fresh();
     f32x16 s[kSub], dp[kSub];
     Frag<T> p[kSub][2], ds[kSub][2];
@@ -854,26 +893,29 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
       else product(f, ds[n][i / 2 / kWide], dk[i / 2 % kWide]);
     };
     auto output_read = [&](int n, int i) { return at.columns(i % 2 == 0 ? gs[buf] : qs[buf], 32 * n + 16 * (i / 2 / kWide), i / 2 % kWide); };
-    uint32_t seen[kSub];
+    // One body for all tiles: bodies that differ by their masks would each keep the sums
+    // in registers of their own.  What is not seen gets a score of -infinity, or, behind a
+    // cap, its weight's bits taken away; a dP there that is not finite makes the row be
+    // done again.
+    uint32_t bits[kSub];
+    auto mask = [&](int n) {
+      bits[n] = ~0u;
+      auto apply = [&](auto which) {
+        Seen<decltype(which)::value, true> seen((begin == INT_MAX ? 1 << 20 : begin - i0) - 32 * n, doc, qd[buf] + 32 * n);
+        if (capped(SC)) bits[n] = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (capped(SC)) bits[n] |= static_cast<uint32_t>(seen(r)) << r;
+          else s[n][r] = seen(r) ? s[n][r] : -INFINITY;
+        }
+      };
+      if (masked && own == nullptr) apply(std::integral_constant<Mask, kEnds>());
+      if (masked && own != nullptr) apply(std::integral_constant<Mask, kIds>());
+    };
     float4 lse, del;
-    auto weight = [&](int n, int r) {  // registers r and r + 1
+    auto weight = [&](int n, int r) {  // registers r and r + 1, in their order
       // the distance |i + off - j| with queries in registers: as if the key stood at j - off
       const ScoreMap<T, SC> map(a, slope2, j - off - i0 - 32 * n);
-      if (masked && r == 0) {
-        seen[n] = 0;
-        const int from = begin == INT_MAX ? INT_MAX : begin - i0 - 32 * n - 4 * half;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) seen[n] |= static_cast<uint32_t>(result_row(x, 0) >= from) << x;
-        if (own != nullptr) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int4 d = *reinterpret_cast<const int4*>(&qd[buf][32 * n + 8 * x + 4 * half]);
-            const uint32_t same = static_cast<uint32_t>(d.x == doc) | static_cast<uint32_t>(d.y == doc) << 1 |
-                                  static_cast<uint32_t>(d.z == doc) << 2 | static_cast<uint32_t>(d.w == doc) << 3;
-            seen[n] &= same << (4 * x) | ~(15u << (4 * x));
-          }
-        }
-      }
       if (r % 4 == 0) {
         lse = *reinterpret_cast<const float4*>(&stats[buf][0][32 * n + 2 * r + 4 * half]);
         del = *reinterpret_cast<const float4*>(&stats[buf][1][32 * n + 2 * r + 4 * half]);
@@ -885,14 +927,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
         float bend;
         const float t = map(s[n][r + y], r + y, bend);
         w[y] = __builtin_amdgcn_exp2f(fmaf(t, map.factor, -ls[y]));
+        if (capped(SC)) w[y] = with_bit(w[y], bits[n], r + y);
         g[y] = w[y] * (dp[n][r + y] - de[y]);
         if (capped(SC)) g[y] *= bend;
         if (std::is_same<T, fp16_t>::value) g[y] *= lift;
-        if (masked) {
-          const bool sees = seen[n] >> (r + y) & 1;
-          w[y] = sees ? w[y] : 0.f;
-          g[y] = sees ? g[y] : 0.f;
-        }
       }
       p[n][r / 8].set2(r % 8, w[0], w[1]);
       ds[n][r / 8].set2(r % 8, g[0], g[1]);
@@ -906,16 +944,22 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
         for (int r = kRows * (i / kEvery); r < kRows * (i / kEvery + 1); r += 2) weight(n, r);
     };
     if constexpr (kSub == 2) {
-      piped<T, 4 * kA, 4>(
-          [&](auto i) { return i < 2 * kA ? score_read(i / kA, i % kA) : output_read(i / kA - 2, i % kA); },
-          [&](auto i, const Frag<T>& f) {
-            if (i < 2 * kA) score(i / kA, i % kA, f);
-            else output(i / kA - 2, i % kA, f);
-            if (i / kA == 1) weights_beside(0, i % kA);
-            if (i / kA == 2) weights_beside(1, i % kA);
-          });
+      piped<T, kA, 4>([&](auto i) { return score_read(0, i); }, [&](auto i, const Frag<T>& f) { score(0, i, f); });
+      mask(0);
+      piped<T, kA, 4>([&](auto i) { return score_read(1, i); },
+                      [&](auto i, const Frag<T>& f) {
+                        score(1, i, f);
+                        weights_beside(0, i);
+                      });
+      mask(1);
+      piped<T, 2 * kB, 4>([&](auto i) { return output_read(i / kB, i % kB); },
+                          [&](auto i, const Frag<T>& f) {
+                            output(i / kB, i % kB, f);
+                            if (i < kB) weights_beside(1, i);
+                          });
     } else {
       piped<T, kA, 4>([&](auto i) { return score_read(0, i); }, [&](auto i, const Frag<T>& f) { score(0, i, f); });
+      mask(0);
 #pragma unroll
       for (int r = 0; r < 16; r += 2) weight(0, r);
       __builtin_amdgcn_sched_barrier(0);
@@ -958,8 +1002,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
       const float slope2 = a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
       bool masked = i < most_begin;
       if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
-      if (masked) step(std::true_type(), i, slope2, buf);
-      else step(std::false_type(), i, slope2, buf);
+      step(masked, i, slope2, buf);
     }
     landed(std::integral_constant<int, 1 - kBuf>());
     i = following;
