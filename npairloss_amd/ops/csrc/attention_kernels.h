@@ -353,10 +353,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
   if (j >= 0) {
     load(j, std::integral_constant<int, 0>());
     landed(std::integral_constant<int, 0>());
-  }
-  while (j >= 0) {
-    turn(std::integral_constant<int, 0>());
-    if (j >= 0) turn(std::integral_constant<int, 1>());
+    do {
+      turn(std::integral_constant<int, 0>());
+      if (j >= 0) turn(std::integral_constant<int, 1>());
+    } while (j >= 0);
   }
 
   const float total = run.l + other_half(run.l);
@@ -770,10 +770,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   if (j >= 0) {
     load(j, std::integral_constant<int, 0>());
     landed(std::integral_constant<int, 0>());
-  }
-  while (j >= 0) {
-    turn(std::integral_constant<int, 0>());
-    if (j >= 0) turn(std::integral_constant<int, 1>());
+    do {
+      turn(std::integral_constant<int, 0>());
+      if (j >= 0) turn(std::integral_constant<int, 1>());
+    } while (j >= 0);
   }
 
   uint32_t again = 0;
@@ -788,10 +788,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
 // them pass by in tiles.
 //   P = 2^(S - lse), dV^T += dO^T P, dS = P (dO V^T - delta) bend, dK^T += Q^T dS
 template <typename T, int DP, Score SC>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void dkv_tiles_kernel(AttnArgs a, const DocRange* ranges, int k_blocks, int splits, float* __restrict__ part) {
-  constexpr int QT = sizeof(T) == 2 ? 64 : 32, kKeys = 32 * kWaves;
-  __shared__ __attribute__((aligned(16))) T qs[2][QT * DP];
-  __shared__ __attribute__((aligned(16))) T gs[2][QT * DP];
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_kernel(AttnArgs a, const DocRange* ranges, int k_blocks, int splits, float* __restrict__ part) {
+  constexpr bool kHalf = sizeof(T) == 2 && DP == 128;
+  constexpr int QT = sizeof(T) == 2 && DP == 64 ? 64 : 32, kKeys = 32 * kWaves;
+  // Width 128 in 16 bits fits two waves a SIMD with V's operands and some of K's in shared
+  // memory, of which two workgroups then fill 149 of 160 KB.
+  constexpr int kSteps = DP / 16, kFromLds = SC == kBoth ? 3 : 2, kInRegs = kSteps - kFromLds;  // of K's operands
+  __shared__ Frag<T> kept[kHalf ? kWaves : 1][kHalf ? kSteps + kFromLds : 1][WAVE];
+  // Names of their own: in one array the compiler takes a read of one buffer for one of the
+  // other's too, and waits for the tile on its way.
+  __shared__ __attribute__((aligned(16))) T qs0[QT * DP], qs1[QT * DP], gs0[QT * DP], gs1[QT * DP];
   __shared__ __attribute__((aligned(16))) float stats[2][2][QT];  // lse, delta
   __shared__ __attribute__((aligned(16))) int qd[2][QT];
   const int t = threadIdx.x, lane = t % WAVE, half = lane / 32;
@@ -813,6 +819,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
   if (a.scale < 0.f) {
 #pragma unroll
     for (int x = 0; x < DP / 16; ++x) kf[x].v = -kf[x].v;
+  }
+  if constexpr (kHalf) {  // a lane's own operands: it reads what it wrote
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) kept[wave][x][lane] = vf[x];
+#pragma unroll
+    for (int x = 0; x < kFromLds; ++x) kept[wave][kSteps + x][lane] = kf[kInRegs + x];
   }
   // the first query that sees a key
   const int prefix = a.prefix != nullptr ? a.prefix[b] : 0;
@@ -877,7 +889,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
   const Reader<T, DP> reader;
   // The scores of 32 queries pass under the weights of the 32 before, and those'
   // products under the weights of these.
-  constexpr int kSub = QT / 32, kSteps = DP / 16, kWide = DP / 32;
+  constexpr int kSub = QT / 32, kWide = DP / 32;
   auto step = [&](bool masked, int i0, float slope2, auto buf) {
     const Reader<T, DP> at = reader.fresh();
     f32x16 s[kSub], dp[kSub];
@@ -887,12 +899,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
       if (i % 2 == 0) product(f, kf[i / 2], s[n]);
       else product(f, vf[i / 2], dp[n]);
     };
-    auto score_read = [&](int n, int i) { return at.rows(i % 2 == 0 ? qs[buf] : gs[buf], 32 * n, i / 2); };
+    auto score_read = [&](int n, int i) { return at.rows(i % 2 == 0 ? (buf == 0 ? qs0 : qs1) : (buf == 0 ? gs0 : gs1), 32 * n, i / 2); };
     auto output = [&](int n, int i, const Frag<T>& f) {
       if (i % 2 == 0) product(f, p[n][i / 2 / kWide], dv[i / 2 % kWide]);
       else product(f, ds[n][i / 2 / kWide], dk[i / 2 % kWide]);
     };
-    auto output_read = [&](int n, int i) { return at.columns(i % 2 == 0 ? gs[buf] : qs[buf], 32 * n + 16 * (i / 2 / kWide), i / 2 % kWide); };
+    auto output_read = [&](int n, int i) { return at.columns(i % 2 == 0 ? (buf == 0 ? gs0 : gs1) : (buf == 0 ? qs0 : qs1), 32 * n + 16 * (i / 2 / kWide), i / 2 % kWide); };
     // One body for all tiles: bodies that differ by their masks would each keep the sums
     // in registers of their own.  What is not seen gets a score of -infinity, or, behind a
     // cap, its weight's bits taken away; a dP there that is not finite makes the row be
@@ -958,7 +970,29 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
                             if (i < kB) weights_beside(1, i);
                           });
     } else {
-      piped<T, kA, 4>([&](auto i) { return score_read(0, i); }, [&](auto i, const Frag<T>& f) { score(0, i, f); });
+      if constexpr (kHalf) {
+        // Q, V, dO a step; K, Q, V, dO where K is not in registers
+        constexpr int kThrees = 3 * kInRegs;
+        int own_lane = lane;
+        asm volatile("" : "+v"(own_lane));
+        s[0] = dp[0] = zeros16();
+        Frag<T> hold;
+        piped<T, kThrees + 4 * kFromLds, 4>(
+            [&](auto i) {
+              constexpr int n = i < kThrees ? i % 3 + 1 : (i - kThrees) % 4, x = i < kThrees ? i / 3 : kInRegs + (i - kThrees) / 4;
+              if constexpr (n == 0) return kept[wave][kSteps + x - kInRegs][own_lane];
+              else if constexpr (n == 2) return kept[wave][x][own_lane];
+              else return at.rows(n == 1 ? (buf == 0 ? qs0 : qs1) : (buf == 0 ? gs0 : gs1), 0, x);
+            },
+            [&](auto i, const Frag<T>& f) {
+              constexpr int n = i < kThrees ? i % 3 + 1 : (i - kThrees) % 4, x = i < kThrees ? i / 3 : kInRegs + (i - kThrees) / 4;
+              if constexpr (n % 2 == 0) hold = f;
+              else if constexpr (n == 1) product(f, x < kInRegs ? kf[x] : hold, s[0]);
+              else product(f, hold, dp[0]);
+            });
+      } else {
+        piped<T, kA, 4>([&](auto i) { return score_read(0, i); }, [&](auto i, const Frag<T>& f) { score(0, i, f); });
+      }
       mask(0);
 #pragma unroll
       for (int r = 0; r < 16; r += 2) weight(0, r);
@@ -979,8 +1013,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
       there = range_next.there >> (i % kDocTile);
       ids = staged_word(d0 + i, t, rows);
     }
-    Flight<T, DP, QT, kWaves>::load(q_row<T>(a, b, i, h), a.qs.l, there, a.D, qs[buf], wave);
-    Flight<T, DP, QT, kWaves>::load(g_row<T>(a, b, i, h), a.gs.l, there, a.D, gs[buf], wave);
+    Flight<T, DP, QT, kWaves, kHalf>::load(q_row<T>(a, b, i, h), a.qs.l, there, a.D, (buf == 0 ? qs0 : qs1), wave);
+    Flight<T, DP, QT, kWaves, kHalf>::load(g_row<T>(a, b, i, h), a.gs.l, there, a.D, (buf == 0 ? gs0 : gs1), wave);
   };
   auto landed = [&](auto buf) {
     const bool here = there >> lane & 1;
@@ -1011,10 +1045,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP == 64 ? 2 : 1) void 
   if (i >= 0) {
     load(i, h, std::integral_constant<int, 0>());
     landed(std::integral_constant<int, 0>());
-  }
-  while (i >= 0) {
-    turn(std::integral_constant<int, 0>());
-    if (i >= 0) turn(std::integral_constant<int, 1>());
+    do {
+      turn(std::integral_constant<int, 0>());
+      if (i >= 0) turn(std::integral_constant<int, 1>());
+    } while (i >= 0);
   }
   const float drop = exp2f(-kWeightLift);
   if (splits > 1) {  // joined, and looked at, by the next kernel

@@ -164,7 +164,8 @@ struct Reader {
 // the swizzle.  Rows without their bit in `there` and chunks behind the width come
 // as zeros (an offset beyond the buffer's end reads as zero).  Nothing waits here:
 // `arrived` does, and the compiler knows of no dependence.
-template <typename T, int DP, int ROWS, int WAVES>
+// FRESH: a lane's offsets are worked out each time, not held over a loop.
+template <typename T, int DP, int ROWS, int WAVES, bool FRESH = false>
 struct Flight {
   using Tl = Tile<T, DP>;
   static constexpr int kStep = WAVES * WAVE / Tl::kChunks;  // rows of one load of all waves
@@ -174,7 +175,8 @@ struct Flight {
   static DEVINL void load(const T* base, int64_t row_stride, uint64_t there, int D, T* tile, int wave) {
     auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7FFFFFFF, 0x00020000);
     const int stride = static_cast<int>(row_stride) * static_cast<int>(sizeof(T));
-    const int place = wave * WAVE + threadIdx.x % WAVE;
+    int place = wave * WAVE + threadIdx.x % WAVE;
+    if (FRESH) asm volatile("" : "+v"(place));
     const int row = place / Tl::kChunks, c = place % Tl::kChunks ^ Tl::swizzle(row);
     const int at = row * stride;
     // full tiles of full rows need no look at every row
@@ -190,10 +192,14 @@ struct Flight {
   }
 };
 
-// All but the last `N` loads of this wave are in shared memory.
+// All but the last `N` loads of this wave are in shared memory.  The builtin and not asm:
+// the compiler then knows that loads into registers have arrived, too, and has no wait
+// of its own for them among the products of a loop.
 template <int N>
 DEVINL void arrived() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);  // vmcnt N, the others as they are
+  asm volatile("" ::: "memory");
 }
 // All reads of shared memory of this wave are in registers.
 DEVINL void read_out() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
