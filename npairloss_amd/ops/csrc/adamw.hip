@@ -320,13 +320,15 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
                       "adamw_step: scales ", i, " are not fp32 [blocks of ", kBlock, ", 2]");
     TORCH_CHECK_VALUE(n < (int64_t{1} << 40), "adamw_step: parameter ", i, " is too large");
   }
-  for (const auto* list : {&params, &steps}) {  // a tensor that comes twice would be updated by two workgroups at once
-    std::vector<const void*> at;
+  const auto lists = {&params, &ms, &vs, &steps, &masters, &scales};
+  std::vector<const void*> written;  // what comes twice would be updated by two workgroups at once
+  for (const auto* list : lists)
     for (const auto& x : *list)
-      if (x.numel() > 0) at.push_back(x.data_ptr());
-    std::sort(at.begin(), at.end());
-    TORCH_CHECK(std::adjacent_find(at.begin(), at.end()) == at.end(), "adamw_step: a tensor comes twice");
-  }
+      if (x.numel() > 0) written.push_back(x.data_ptr());
+  std::sort(written.begin(), written.end());
+  TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), "adamw_step: a tensor comes twice");
+  for (const auto* list : lists)  // a graph that has saved one of them learns of the change
+    for (const auto& x : *list) x.unsafeGetTensorImpl()->bump_version();
   at::DeviceGuard guard(device);
   for (size_t i = 0; i < count; ++i)  // gradients in another order of dimensions are brought into the parameter's
     if (!like(grads[i], params[i])) grads[i] = torch::empty_like(params[i]).copy_(grads[i]);

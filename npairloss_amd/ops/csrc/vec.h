@@ -47,13 +47,6 @@ DEVINL uint32_t pack_fp8(float a, float b, float c, float d) {
 // The larger of two magnitudes; NaN if one of them is.
 DEVINL float max_or_nan(float a, float b) { return (a > b || a != a) ? a : b; }
 
-template <int N>
-DEVINL float group_max_or_nan(float v) {  // over N neighbouring lanes, N a power of two
-#pragma unroll
-  for (int off = N / 2; off > 0; off >>= 1) v = max_or_nan(v, __shfl_xor(v, off, WAVE));
-  return v;
-}
-
 // Runs `fn` with a value of the element type that `dtype` names.
 #define DISPATCH_FLOAT(dtype, NAME, ...)                                   \
   [&] {                                                                    \

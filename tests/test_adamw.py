@@ -177,7 +177,7 @@ def test_layouts(bits, device):
 
 @pytest.mark.parametrize("device", DEVICES)
 def test_many_tensors(device):
-    """More than one launch takes, counts that differ, one captured by none."""
+    """More tensors than one launch takes, with counts of steps that differ."""
     sizes = [(1 + 13 * i % 700,) for i in range(470)]
     params, grads, states = make(sizes, torch.float32, device, 32, False)
     for i, s in enumerate(states):
@@ -226,6 +226,21 @@ def test_the_same_tensor_twice_is_refused():
     more[2][0]["step"] = states[0]["step"]
     with pytest.raises(RuntimeError, match="twice"):
         call(params + more[0], grads + more[1], states + more[2])
+    for name in ("exp_avg", "exp_avg_sq"):
+        more = make([(300,)], torch.float32, "cuda", 32, False)
+        more[2][0][name] = states[0][name]
+        with pytest.raises(RuntimeError, match="twice"):
+            call(params + more[0], grads + more[1], states + more[2])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_graph_that_saved_a_parameter_learns_of_the_step(device):
+    w = torch.randn(40, device=device, requires_grad=True)
+    loss = (w * w).sum()
+    state = adamw_state(w)
+    adamw_step([w], [torch.ones_like(w)], [state["exp_avg"]], [state["exp_avg_sq"]], [state["step"]], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
 
 
 @pytest.mark.parametrize("device", DEVICES)
