@@ -47,14 +47,20 @@ DEVINL int causal_end(const AttnArgs& a, int b, int i) {
 
 DEVINL bool seen_by_documents(int dq, int dk) { return dq == dk && dk >= 0; }
 
-// The cap as c tanh(s / c) = c - 2 c u with u = 1 / (1 + 2^(2 log2(e) s / c)), and its
-// derivative 1 - tanh^2 = 4 u (1 - u): an exponential and a reciprocal, each a unit
-// or so off, under 8 units of c together.  fp32 takes the library's exponential and
-// a true quotient.
-template <typename T> DEVINL float cap_share(float s_over_c) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * s_over_c));
+// c tanh(x) and the derivative of tanh at x.  16-bit types: with u = 1 / (1 + 2^(2 log2(e) x))
+// they are c - 2 c u and 4 u (1 - u), an exponential and a reciprocal, each a unit or so off:
+// under 8 units of c together, which with c <= 1024 is half a step of an fp16 weight.  fp32
+// takes the library's tanh, whose error is relative to the value.
+template <typename T> DEVINL float cap(float x, float c, float& bend) {
+  const float u = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * x));
+  bend = 4.f * fmaf(-u, u, u);
+  return fmaf(-2.f * c, u, c);
 }
-template <> DEVINL float cap_share<float>(float s_over_c) { return 1.f / (1.f + expf(2.f * s_over_c)); }
+template <> DEVINL float cap<float>(float x, float c, float& bend) {
+  const float t = tanhf(x);
+  bend = (1.f - t) * (1.f + t);
+  return c * t;
+}
 
 template <typename T>
 DEVINL float dot_row(const T* __restrict__ x, const T* __restrict__ y, int D) {
@@ -74,11 +80,7 @@ template <typename T>
 DEVINL float transformed(const AttnArgs& a, float dot, float slope, int distance, float* bend) {
   float s = dot * a.scale;
   *bend = 1.f;
-  if (a.softcap > 0.f) {
-    const float u = cap_share<T>(s / a.softcap);
-    s = a.softcap - 2.f * a.softcap * u;
-    *bend = 4.f * u * (1.f - u);
-  }
+  if (a.softcap > 0.f) s = cap<T>(s / a.softcap, a.softcap, *bend);
   return (s - slope * static_cast<float>(distance)) * kLog2e;
 }
 

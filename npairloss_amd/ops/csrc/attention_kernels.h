@@ -58,9 +58,7 @@ struct ScoreMap {
     bend = 1.f;
     if (SC == kPlain) return s;
     if (capped(SC)) {
-      const float u = cap_share<T>(s * in);
-      bend = 4.f * fmaf(-u, u, u);
-      s = fmaf(-2.f * out, u, out);
+      s = cap<T>(s * in, out, bend);
     } else {
       s *= in;
     }

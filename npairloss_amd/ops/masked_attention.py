@@ -26,6 +26,7 @@ from . import _backend
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 MAX_WIDTH = 128
+MIN_SOFTCAP, MAX_SOFTCAP_16, MAX_SOFTCAP_32 = 2.0 ** -20, 2.0 ** 10, 2.0 ** 20
 
 
 # ---------------------------------------------------------------------------
@@ -137,7 +138,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     h // (heads / key heads).  fp32, bf16 or fp16, widths up to 128, any strides;
     differentiable in q, k and v.
 
-    `scale` is width^-0.5 by default.  `softcap` 0 leaves scores as they are.
+    `scale` is width^-0.5 by default.  `softcap` 0 leaves scores as they are; others
+    lie from 2^-20 to 2^20 (16-bit types: 2^10, as the cap is formed to 8 units of it).
     `slopes` fp32 [heads] biases by distance (no gradient).  `causal` hides keys
     behind the query's place, but for the first `prefix[b]` (int32 [batch]) keys.
     `documents` int32 [batch, queries] and `key_documents` [batch, keys] (the same
@@ -158,8 +160,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     if Hk == 0 or H % Hk:
         raise ValueError(f"attention: {Hk} key heads do not divide {H} heads")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale) or not 0.0 <= float(softcap) < math.inf:
-        raise ValueError(f"attention: finite scale and softcap >= 0 expected, got {scale}, {softcap}")
+    if not abs(scale) <= 2.0 ** 100:
+        raise ValueError(f"attention: a scale of at most 2^100 expected, got {scale}")
+    most = MAX_SOFTCAP_32 if q.dtype == torch.float32 else MAX_SOFTCAP_16
+    if not (softcap == 0.0 or MIN_SOFTCAP <= softcap <= most):
+        raise ValueError(f"attention: a softcap of 0 or {MIN_SOFTCAP:g} to {most:g} expected for {q.dtype}, got {softcap}")
     if slopes is not None:
         if slopes.shape != (H,) or slopes.dtype != torch.float32:
             raise ValueError(f"attention: slopes are fp32 [{H}], got {slopes.dtype} {tuple(slopes.shape)}")

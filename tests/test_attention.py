@@ -285,6 +285,59 @@ def test_refusals(device):
         attention(wide, wide, wide)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_refused_scales_and_caps(device):
+    q = torch.randn(1, 4, 2, 16, device=device)
+    for more in (dict(scale=1e200), dict(scale=-math.inf), dict(softcap=1e-7), dict(softcap=2.0 ** 21), dict(softcap=math.nan)):
+        with pytest.raises(ValueError):
+            attention(q, q, q, **more)
+    h = q.half()
+    with pytest.raises(ValueError):
+        attention(h, h, h, softcap=1025.0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_far_caps(dtype, device):
+    """A cap far over the scores changes them by s^3 / (3 c^2), here under 2^-30."""
+    q, k, v, dout, more = inputs(case(Lq=70, H=2, D=64, causal=True), dtype, device)
+    got = run(q, k, v, dout, more | dict(softcap=2.0 ** 20 if dtype == torch.float32 else 2.0 ** 10))
+    if dtype == torch.float32:
+        # the cap adds a product, tanh (2 units) and a product to a score, 6 units at most; that is
+        # under what the uncapped score's sum and exponent are counted with, so twice their tolerance
+        want, tol = exact(q, k, v, dout, more | dict(softcap=0.0), dtype)
+        tol = {n: 2 * x for n, x in tol.items()}
+    else:
+        want, tol = exact(q, k, v, dout, more | dict(softcap=2.0 ** 10), dtype)
+    for n in want:
+        assert_within(got[n], want[n], tol[n], n)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["causal", "documents", "documents, mixed", "prefix", "uneven", "documents, one query", "width 128"])
+def test_no_scale_and_a_negative_one(name, dtype, device):
+    """scale -c is scale c with -q, the gradient of q turned: scores, weights and the products
+    summed for out, dq and dv are the same numbers, so these are equal bit for bit.  For dk the
+    products have the other sign, and how a matrix instruction rounds its fp32 sum need not be
+    the same for both signs: it stays within what the formula's sum may be off by.  scale 0 gives
+    what is seen equal weights (and q, k no gradient)."""
+    c = CASES[name]
+    q, k, v, dout, more = inputs(c, dtype, device)
+    more = more | dict(scale=0.2)
+    got, want = run(q, k, v, dout, more | dict(scale=-0.2)), run(-q, k, v, dout, more)
+    for n in ("out", "dq", "dv"):
+        assert torch.equal(got[n], -want[n] if n == "dq" else want[n]), n
+    want, tol = exact(-q, k, v, dout, more, dtype)
+    assert_within(got["dk"], want["dk"], tol["dk"], "dk")
+    more = {n: x for n, x in more.items() if n not in ("slopes", "softcap")} | dict(scale=0.0)
+    got = run(q, k, v, dout, more)
+    assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
+    want, tol = exact(torch.zeros_like(q), k, v, dout, more | dict(scale=1.0), dtype)
+    for n in ("out", "dv"):
+        assert_within(got[n], want[n], tol[n], n)
+
+
 @pytest.mark.gpu
 def test_captured():
     """Forward and backward replayed; two graphs of one call do not share their workspaces' contents."""
