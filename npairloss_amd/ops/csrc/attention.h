@@ -31,6 +31,8 @@ struct AttnArgs {
   const int* prefix;     // [B] or null
   const int* q_doc;      // [B, Lq] or null
   const int* k_doc;      // [B, Lk] or null
+  const int* q_order;    // [B, blocks of 128 queries] or null: the order to take them in
+  const int* k_order;    // the same of keys
   // backward
   const void* dout; RowStrides gs;
   float* delta;          // [B, H, Lq]: sum_d dout o

@@ -20,6 +20,42 @@ __global__ __launch_bounds__(WAVE) void doc_ranges_kernel(const int* __restrict_
   if (threadIdx.x == 0) out[blockIdx.x] = DocRange{lo, hi, there};
 }
 
+// Blocks of kBlockRows rows in falling order of how many tiles of the other side their ids
+// may meet, for each batch row: with packed documents one block has ten times the work of
+// another, and the long ones have to begin first.  Two rows of 4096 tokens, 12 heads of 64
+// bf16, images of 37 to 785 tokens: dQ 124 -> 82 us, dK and dV 143 -> 95, forward 88 -> 77,
+// for 7 us of this kernel a direction.
+constexpr int kBlockRows = 2 * kDocTile, kMostOrdered = 1024;
+
+__global__ __launch_bounds__(kMostOrdered) void block_order_kernel(const DocRange* __restrict__ own, int own_tiles, const DocRange* __restrict__ other,
+                                                                   int other_tiles, int blocks, int* __restrict__ order) {
+  __shared__ int2 staged[kMostOrdered];
+  __shared__ int counts[kMostOrdered];
+  const int t = threadIdx.x, b = blockIdx.x;
+  own += static_cast<int64_t>(b) * own_tiles;
+  other += static_cast<int64_t>(b) * other_tiles;
+  int lo = INT_MAX, hi = -1, count = 0;
+  for (int x = 2 * t; x < min(2 * t + 2, own_tiles); ++x) {
+    lo = min(lo, own[x].lo);
+    hi = max(hi, own[x].hi);
+  }
+  for (int base = 0; base < other_tiles; base += blockDim.x) {
+    const int n = min(static_cast<int>(blockDim.x), other_tiles - base);
+    __syncthreads();
+    if (t < n) staged[t] = make_int2(other[base + t].lo, other[base + t].hi);
+    __syncthreads();
+#pragma unroll 8
+    for (int x = 0; x < n; ++x) count += staged[x].x <= hi && staged[x].y >= lo;
+  }
+  counts[t] = count;
+  __syncthreads();
+  if (t >= blocks) return;
+  int rank = 0;
+#pragma unroll 8
+  for (int x = 0; x < blocks; ++x) rank += counts[x] > count || (counts[x] == count && x < t);
+  order[static_cast<int64_t>(b) * blocks + rank] = t;
+}
+
 void check_tensor(const torch::Tensor& x, const torch::Tensor& q, const char* name) {
   const int64_t per16 = 16 / x.element_size();
   TORCH_CHECK(x.is_cuda() && x.device() == q.device() && x.dim() == 4 && x.scalar_type() == q.scalar_type(),
@@ -85,6 +121,29 @@ const DocRange* ranges_of(const torch::Tensor& x) {
   return x.defined() ? reinterpret_cast<const DocRange*>(x.data_ptr<int>()) : nullptr;
 }
 
+// The order of a side's blocks, or nothing where there is none to choose or so many that
+// they even out by themselves.
+torch::Tensor block_order(const torch::Tensor& own, int own_rows, const torch::Tensor& other, int other_rows, int B, hipStream_t stream) {
+  const int blocks = (own_rows + kBlockRows - 1) / kBlockRows;
+  if (!own.defined() || blocks < 2 || blocks > kMostOrdered) return torch::Tensor();
+  auto out = torch::empty({B, blocks}, own.options());
+  block_order_kernel<<<B, (blocks + WAVE - 1) / WAVE * WAVE, 0, stream>>>(
+      ranges_of(own), (own_rows + kDocTile - 1) / kDocTile, ranges_of(other), (other_rows + kDocTile - 1) / kDocTile, blocks, out.data_ptr<int>());
+  HIP_CHECK_LAST();
+  return out;
+}
+
+const int* order_of(const torch::Tensor& x) { return x.defined() ? x.data_ptr<int>() : nullptr; }
+
+// The ids of both sides by tiles; one tensor for both stays one.
+struct Ranges {
+  torch::Tensor k, q;
+  Ranges(const AttnArgs& a, const c10::optional<torch::Tensor>& q_doc, const c10::optional<torch::Tensor>& k_doc, bool both, hipStream_t stream) {
+    k = doc_ranges(k_doc, a.B, a.Lk, stream);
+    if (both) q = a.q_doc == a.k_doc && a.Lq == a.Lk ? k : doc_ranges(q_doc, a.B, a.Lq, stream);
+  }
+};
+
 }  // namespace
 
 // {o [B, Lq, H, D], lse [B, H, Lq], what rounding took from o (16-bit types, if `keep_rest`) or nothing}
@@ -102,8 +161,11 @@ std::vector<torch::Tensor> attention_fwd(torch::Tensor q, torch::Tensor k, torch
   a.o = o.data_ptr();
   a.lse = lse.data_ptr<float>();
   auto stream = at::hip::getCurrentHIPStream();
-  const auto ranges = doc_ranges(k_doc, a.B, a.Lk, stream);
-  DISPATCH_FLOAT(q.scalar_type(), "attention", [&] { attention_forward<T>(a, ranges_of(ranges), q.options(), stream); });
+  const bool tiled = attention_in_tiles(a);
+  const Ranges ranges(a, q_doc, k_doc, tiled, stream);
+  const auto order = tiled ? block_order(ranges.q, a.Lq, ranges.k, a.Lk, a.B, stream) : torch::Tensor();
+  a.q_order = order_of(order);
+  DISPATCH_FLOAT(q.scalar_type(), "attention", [&] { attention_forward<T>(a, ranges_of(ranges.k), q.options(), stream); });
   HIP_CHECK_LAST();
   return {o, lse, rest};
 }
@@ -130,12 +192,17 @@ std::vector<torch::Tensor> attention_bwd(torch::Tensor dout, torch::Tensor q, to
   a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
   auto stream = at::hip::getCurrentHIPStream();
-  const auto k_ranges = doc_ranges(k_doc, a.B, a.Lk, stream), q_ranges = doc_ranges(q_doc, a.B, a.Lq, stream);
+  const Ranges ranges(a, q_doc, k_doc, true, stream);
+  const bool one = ranges.q.is_same(ranges.k);
+  const auto q_order = block_order(ranges.q, a.Lq, ranges.k, a.Lk, a.B, stream);
+  const auto k_order = one ? q_order : block_order(ranges.k, a.Lk, ranges.q, a.Lq, a.B, stream);
+  a.q_order = order_of(q_order);
+  a.k_order = order_of(k_order);
   torch::Tensor top;  // filled by a kernel: a captured graph clears it at every replay
   if (q.scalar_type() == at::kHalf) top = torch::zeros({1}, q.options().dtype(at::kInt));
   a.grad_top = top.defined() ? reinterpret_cast<unsigned*>(top.data_ptr<int>()) : nullptr;
   DISPATCH_FLOAT(q.scalar_type(), "attention", [&] {
-    attention_backward<T>(a, ranges_of(k_ranges), ranges_of(q_ranges), q.options(), stream);
+    attention_backward<T>(a, ranges_of(ranges.k), ranges_of(ranges.q), q.options(), stream);
   });
   HIP_CHECK_LAST();
   return {dq, dk, dv};

@@ -12,6 +12,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / WAVE;
 constexpr int kQueries = 32 * kWaves;  // of a workgroup of the tiled kernels
+static_assert(kQueries == 2 * kDocTile, "blocks of rows are ordered by pairs of tiles");
 
 // The keys before which the query of a lane sees any (0: none), and its id.
 struct Query {
@@ -263,8 +264,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
   const int t = threadIdx.x, lane = t % WAVE;
   const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
   const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
-  const int64_t bh = linear / q_tiles;
-  const int i0 = tile_at(linear % q_tiles, q_tiles, bh, a.causal && a.k_doc == nullptr) * kQueries;
+  int64_t bh = linear / q_tiles;
+  int i0 = tile_at(linear % q_tiles, q_tiles, bh, a.causal && a.k_doc == nullptr) * kQueries;
+  if (a.q_order != nullptr) i0 = ordered(a.q_order, linear, q_tiles, a.B, a.H, bh) * kQueries;
   const int b = bh / a.H, h = bh % a.H, kv = h / (a.H / a.Hk);
   const int i = i0 + 32 * wave + lane % 32;
   const bool ok = i < a.Lq;
@@ -278,6 +280,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
   // rows that are not there decide nothing, and nothing of them is kept
   const int least_end = wave_min(ok ? q.end : INT_MAX), most_end = wave_max(q.end);
   const int doc_lo = wave_min(ok ? q.doc : INT_MAX), doc_hi = wave_max(ok ? q.doc : INT_MIN);
+  const int doc_least = doc_lo >= 0 ? doc_lo : wave_min(ok && q.doc >= 0 ? q.doc : INT_MAX);
 
   int lo = 0, hi = 0;  // ids of the workgroup's queries
   if (ranges != nullptr) {
@@ -340,7 +343,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
     const int following = next();
     const DocRange present = range;
     if (following >= 0) load(following, std::integral_constant<int, 1 - kBuf>());
-    if (j < most_end) {
+    if (j < most_end && (own == nullptr || (present.lo <= doc_hi && present.hi >= doc_least))) {
       bool masked = j + KT > least_end;
       if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
       run.template absorb<SC>(a, at, qf, ks[kBuf], vs[kBuf], kd[kBuf], q, j, !masked ? kSeen : own == nullptr ? kEnds : kIds);
@@ -576,8 +579,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   const int t = threadIdx.x, lane = t % WAVE;
   const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
   const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
-  const int64_t bh = linear / q_tiles;
-  const int i0 = tile_at(linear % q_tiles, q_tiles, bh, a.causal && a.k_doc == nullptr) * kQueries;
+  int64_t bh = linear / q_tiles;
+  int i0 = tile_at(linear % q_tiles, q_tiles, bh, a.causal && a.k_doc == nullptr) * kQueries;
+  if (a.q_order != nullptr) i0 = ordered(a.q_order, linear, q_tiles, a.B, a.H, bh) * kQueries;
   const int b = bh / a.H, h = bh % a.H, kv = h / (a.H / a.Hk);
   const int i = i0 + 32 * wave + lane % 32;
   const bool ok = i < a.Lq;
@@ -621,6 +625,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   // rows that are not there decide nothing, and nothing of them is kept
   const int least_end = wave_min(ok ? q.end : INT_MAX), most_end = wave_max(q.end);
   const int doc_lo = wave_min(ok ? q.doc : INT_MAX), doc_hi = wave_max(ok ? q.doc : INT_MIN);
+  const int doc_least = doc_lo >= 0 ? doc_lo : wave_min(ok && q.doc >= 0 ? q.doc : INT_MAX);
   int lo = 0, hi = 0;
   if (ranges != nullptr) {
     lo = INT_MAX, hi = -1;
@@ -757,7 +762,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
     const int following = next();
     const DocRange present = range;
     if (following >= 0) load(following, std::integral_constant<int, 1 - kBuf>());
-    if (j < most_end) {
+    if (j < most_end && (own == nullptr || (present.lo <= doc_hi && present.hi >= doc_least))) {
       bool masked = j + KT > least_end;
       if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
       step(masked, j, buf);
@@ -802,11 +807,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
   const int wave = __builtin_amdgcn_readfirstlane(t / WAVE);
   const int64_t linear = xcd_order(blockIdx.x, gridDim.x);
   const int split = linear % splits;
-  const int64_t bc = linear / splits / k_blocks;
+  int64_t bc = linear / splits / k_blocks;
   // under a causal mask first, last, second, ..: the first blocks have the most queries,
   // and an XCD has a stretch of this order
   const int place = static_cast<int>(linear / splits % k_blocks);
-  const int j0 = (!a.causal || a.k_doc != nullptr ? tile_at(place, k_blocks, bc, false) : place % 2 == 0 ? place / 2 : k_blocks - 1 - place / 2) * kKeys;
+  int j0 = (!a.causal || a.k_doc != nullptr ? tile_at(place, k_blocks, bc, false) : place % 2 == 0 ? place / 2 : k_blocks - 1 - place / 2) * kKeys;
+  if (a.k_order != nullptr) j0 = ordered(a.k_order, linear / splits, k_blocks, a.B, a.Hk, bc) * kKeys;
   const int b = bc / a.Hk, kv = bc % a.Hk, group = a.H / a.Hk, off = a.Lk - a.Lq;
   const int j = j0 + 32 * wave + lane % 32;
   const int doc = j < a.Lk && a.k_doc != nullptr ? a.k_doc[static_cast<int64_t>(b) * a.Lk + j] : 0;
@@ -829,6 +835,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
   const int begin = !ok ? INT_MAX : !a.causal || j < prefix ? 0 : max(0, j - off);
   const int least_begin = wave_min(begin), most_begin = wave_max(begin);
   const int doc_lo = wave_min(doc), doc_hi = wave_max(doc);
+  const int doc_least = doc_lo >= 0 ? doc_lo : wave_min(ok && doc >= 0 ? doc : INT_MAX);
   int lo = 0, hi = 0;
   if (ranges != nullptr) {
     lo = INT_MAX, hi = -1;
@@ -1030,7 +1037,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
     const int following = next(h_next);
     const DocRange present = range;
     if (following >= 0) load(following, h_next, std::integral_constant<int, 1 - kBuf>());
-    if (i + QT > least_begin) {
+    if (i + QT > least_begin && (own == nullptr || (present.lo <= doc_hi && present.hi >= doc_least))) {
       const float slope2 = a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.f;
       bool masked = i < most_begin;
       if (own != nullptr) masked = masked || !(present.one() && doc_lo == doc_hi && present.lo == doc_lo);
@@ -1118,12 +1125,10 @@ void with_variant(const AttnArgs& a, Fn fn) {
   else by_score(std::integral_constant<int, 128>());
 }
 
-// Tiles of queries where they fill the chip and their 128 rows are mostly there; 32
-// rows and stretches of keys where not.
 template <typename T, int DP, Score SC>
 void run_forward(const AttnArgs& a, const DocRange* ranges, const torch::TensorOptions& options, hipStream_t stream) {
   const int64_t tiles = static_cast<int64_t>(a.B) * a.H * ((a.Lq + kQueries - 1) / kQueries);
-  if (tiles >= kComputeUnits && a.Lq >= 64) {
+  if (attention_in_tiles(a)) {
     forward_tiles_kernel<T, DP, SC><<<blocks_for(tiles, 1), kThreads, 0, stream>>>(a, ranges, (a.Lq + kQueries - 1) / kQueries);
     return;
   }

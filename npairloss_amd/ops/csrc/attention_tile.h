@@ -214,6 +214,15 @@ DEVINL int tile_at(int i, int n, int64_t head, bool longest_first) {
   return (i + turn) % n;
 }
 
+// The same with blocks of rows in an order of their own, [B, n], longest first: an XCD's
+// heads, which neighbour in `place`, go through it side by side.  Sets `head`.
+DEVINL int ordered(const int* order, int64_t place, int n, int B, int heads, int64_t& head) {
+  const int64_t all = static_cast<int64_t>(B) * heads, side = all % 8 == 0 ? all / 8 : 1;
+  const int64_t first = place / (side * n), in = place % (side * n);
+  head = first * side + in % side;
+  return order[head / heads * n + in / side];
+}
+
 // One word a thread, the first `n` of them, on the same way.
 DEVINL uint32_t staged_word(const void* base, int t, int n) {
   auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);

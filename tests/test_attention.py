@@ -253,6 +253,20 @@ def test_strides(dtype, device):
     assert all(torch.equal(got[n], base[n]) for n in base)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,L", [(1, 1, 131200), (1, 1, 65600), (2, 16, 1100), (3, 5, 2300)])
+def test_many_documents(B, H, L):
+    """Documents of 50 tokens in long rows are as many batch rows of 50: blocks that are taken in
+    an order of their own, and more of them than are ordered."""
+    n = 50
+    q, k, v, dout, more = inputs(case(B=B * L // n, Lq=n, H=H, D=16, causal=True), torch.bfloat16, "cuda")
+    ids = torch.arange(L // n, dtype=torch.int32, device="cuda").repeat_interleave(n).expand(B, L).contiguous()
+    got = run(*(x.view(B, L, H, 16) for x in (q, k, v, dout)), more | dict(documents=ids))
+    want, tol = exact(q, k, v, dout, more, torch.bfloat16)
+    for name in want:
+        assert_within(got[name].view_as(want[name]), want[name], tol[name], name)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_empty(device):
     for B, Lq, Lk, H in ((0, 3, 3, 2), (2, 0, 3, 2), (2, 3, 0, 2), (2, 0, 0, 2)):
