@@ -3,7 +3,10 @@
 // over a token 3, and a Python function forward and backward takes 40 and more.
 
 #include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 
+#include <initializer_list>
 #include <vector>
 
 std::vector<torch::Tensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual,
@@ -33,6 +36,20 @@ OptTensor opt(const Tensor& x) { return x.defined() ? OptTensor(x) : c10::nullop
 
 void once(const char* name) {  // under create_graph=True the engine records what a backward does
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its gradient has no gradient");
+}
+
+// A leaf whose gradient is still to be added to by a living eager graph has that graph's
+// stream; a captured backward pass would wait across to it, and instantiating such a graph
+// ends the process.
+void capturable(std::initializer_list<OptTensor> leaves, const char* name) {
+  if (!at::GradMode::is_enabled() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const auto& x : leaves) {
+    if (!x.has_value() || !x->requires_grad() || !x->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*x);
+    const auto stream = node ? node->stream() : c10::nullopt;
+    TORCH_CHECK(!stream.has_value() || stream->id() == at::hip::getCurrentHIPStream(x->device().index()).id(), name,
+                ": captured while an eager graph of the same leaf lives on another stream: drop its outputs first");
+  }
 }
 
 Tensor rows(const Tensor& x) {
@@ -158,6 +175,7 @@ struct Attention : torch::autograd::Function<Attention> {
 
 std::vector<Tensor> rms_norm(Tensor x, Tensor weight, OptTensor residual, double eps) {
   check_norm(x, weight, residual);
+  capturable({x, weight, residual}, "rms_norm");
   return RmsNorm::apply(x, weight, residual, eps);
 }
 
@@ -206,6 +224,7 @@ std::vector<Tensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor frequ
                     "rotary: positions ", positions.sizes(), " do not fit q ", q.sizes(), " and frequencies ", frequencies.sizes());
   for (const Tensor& x : {k.value_or(q), positions, frequencies})
     TORCH_CHECK_VALUE(x.device() == q.device(), "rotary: tensors on ", q.device(), " and ", x.device());
+  capturable({q, k}, "rotary");
   if (!axes) positions = positions.unsqueeze(-1);
   if (lead == 1) positions = positions.unsqueeze(0).expand({q.size(0), q.size(1), positions.size(-1)});
   return Rotary::apply(q, k, positions, frequencies.is_contiguous() ? frequencies : frequencies.contiguous(), interleaved, amplitude);
@@ -214,5 +233,6 @@ std::vector<Tensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor frequ
 Tensor attention(Tensor q, Tensor k, Tensor v, double scale, double softcap, OptTensor slopes, bool causal, OptTensor prefix,
                  OptTensor q_doc, OptTensor k_doc) {
   const bool train = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  capturable({q, k, v}, "attention");
   return Attention::apply(q, k, v, scale, softcap, slopes, causal, prefix, q_doc, k_doc, train);
 }

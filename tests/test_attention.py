@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from npairloss_amd.ops import attention
+from npairloss_amd.ops import attention, rms_norm, rotary, rotary_frequencies
 from transformer_util import DEVICES, TYPES, U, assert_within, half_step, least, replays
 
 
@@ -363,6 +363,27 @@ def test_captured():
     alone = attention(*one[:3], **one[4])
     for out in replays(lambda: attention(*one[:3], **one[4])):
         assert torch.equal(out, alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["attention", "rotary", "rms_norm"])
+def test_capture_beside_an_eager_graph_is_refused(name):
+    """A living eager graph of the same leaf: refused before anything is recorded.  Without it
+    the call is captured."""
+    q, k, v, dout, more = inputs(case(Lq=40, H=2, D=16), torch.bfloat16, "cuda")
+    x, w = q.clone().requires_grad_(), torch.ones(16, device="cuda")
+    at, turns = torch.arange(40, device="cuda"), rotary_frequencies(16, device="cuda")[0]
+    call = {"attention": lambda: attention(x, k, v), "rotary": lambda: rotary(x, None, at, turns), "rms_norm": lambda: rms_norm(x, w)}[name]
+    held = call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            call()
+    want = torch.autograd.grad(held, x, dout)[0]
+    del held, graph
+    for out in replays(lambda: torch.autograd.grad(call(), x, dout)[0]):
+        assert torch.equal(out, want)
 
 
 @pytest.mark.gpu
