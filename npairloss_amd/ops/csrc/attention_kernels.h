@@ -255,6 +255,13 @@ DEVINL uint32_t bad_columns(bool bad) {
 template <typename T>
 DEVINL bool repairs(const AttnArgs& a) { return std::is_same<T, fp16_t>::value || a.causal || a.k_doc != nullptr; }
 
+// 32 queries a wave: S^T = K Q^T with lanes as queries, so that a row's maximum and sum stay
+// in a lane and its half, and P^T is the operand of O^T = V^T P^T as it lies.  128 queries a
+// workgroup read each key tile once; two tiles in shared memory, one in use, and three
+// workgroups of width 64 a CU (two of 128).  Bound by the vector units at width 64 (an
+// exponential and seven more instructions a score; 48% of the time, products 15%), which a
+// wave's waits leave idle, and by the products at width 128.  64 images of 197 tokens, 12
+// heads of 64 bf16: 37 us; 8191 tokens, 16 heads of 128 fp16, causal: 390 us, 705 TFLOP/s.
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void forward_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
   constexpr int KT = sizeof(T) == 2 ? 64 : 32, NS = KT / 32;
@@ -399,10 +406,11 @@ DEVINL void finish_row(const AttnArgs& a, int b, int i, int h, float o0, float o
 
 // Few queries: a workgroup takes 32 rows (queries of all heads that share a key
 // head) and a stretch of keys, its waves every fourth 32 keys of it, each with
-// shared memory of its own, so that nothing waits but for its own loads: while one
-// tile is used the next is on its way in registers.  The waves join at the end;
-// where keys are split over workgroups too, `part` [splits, rows, DP] and `stats`
-// (maximum, sum) go to the joining kernel.
+// shared memory of its own, so that nothing waits but for its own loads: as soon as the
+// scores have read K's tile the next is on its way to its place.  The waves join at the
+// end; where keys are split over workgroups too, `part` [splits, rows, DP] and `stats`
+// (maximum, sum) go to the joining kernel.  Bound by memory: 16 caches of up to 65536 keys, 8
+// key heads of 128 bf16, are read at 4.9 TB/s (405 us, as fast as a large copy).
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_split_kernel(
     AttnArgs a, const DocRange* ranges, int row_tiles, int splits, int keys_per_split, float* __restrict__ part, float2* __restrict__ stats) {
@@ -570,6 +578,9 @@ DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(-static_cast<float
 // dQ of 32 queries a wave, and delta for both: lanes are queries, K and V pass by in
 // tiles.
 //   P^T = 2^(S^T - lse), dS^T = P^T (V dO^T - delta) bend, dQ^T += K^T dS^T
+// A kernel of its own and not sums of dK's workgroups into dQ: those would have to be atomic,
+// in an order that changes, or another pass.  It costs two of seven products.  64 images of 197 tokens, 12 heads of 64 bf16: 47 us; 8191 tokens, 16 heads of
+// 128 fp16, causal: 460 us, 900 TFLOP/s, of 1087 in a large library product.
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
   constexpr int KT = sizeof(T) == 2 && DP == 64 ? 64 : 32;
@@ -790,12 +801,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
 // dK and dV of 32 keys a wave: lanes are keys, Q and dO of all heads that share
 // them pass by in tiles.
 //   P = 2^(S - lse), dV^T += dO^T P, dS = P (dO V^T - delta) bend, dK^T += Q^T dS
+// Bound by registers: both sums, and K's and V's operands, are 192 of a wave's 256 at width
+// 128, and what is left sets how far reads and weights go ahead of the products.  64 images of
+// 197 tokens, 12 heads of 64 bf16: 53 us; 8191 tokens, 16 heads on 4 of 128 fp16, causal:
+// 790 us, 700 TFLOP/s, of 1087 in a large library product, and 60 us for the join of eight
+// parts (4.5 TB/s).
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_kernel(AttnArgs a, const DocRange* ranges, int k_blocks, int splits, float* __restrict__ part) {
   constexpr bool kHalf = sizeof(T) == 2 && DP == 128;
   constexpr int QT = sizeof(T) == 2 && DP == 64 ? 64 : 32, kKeys = 32 * kWaves;
   // Width 128 in 16 bits fits two waves a SIMD with V's operands and some of K's in shared
-  // memory, of which two workgroups then fill 149 of 160 KB.
+  // memory, of which two workgroups then fill 149 (kBoth: 157) of 160 KB: 957 us where one
+  // wave with 420 registers took 1057 (8191 tokens, 16 heads on 4, fp16).
   constexpr int kSteps = DP / 16, kFromLds = SC == kBoth ? 3 : 2, kInRegs = kSteps - kFromLds;  // of K's operands
   __shared__ Frag<T> kept[kHalf ? kWaves : 1][kHalf ? kSteps + kFromLds : 1][WAVE];
   // Names of their own: in one array the compiler takes a read of one buffer for one of the

@@ -15,6 +15,11 @@
 // so that it fits in at most 32 registers a thread.  Rows whose width or address is
 // not a multiple of eight elements take the same kernels with one element to
 // an access, neighbouring lanes on neighbouring elements.
+//
+// 12608 rows of 768 bf16 with a residual: 15.5 us forward (5.0 TB/s), 22.8 and 3.9 backward
+// (3.4 TB/s: a workgroup walks over rows to keep the weight's gradient in registers, and each
+// waits for its row); 16384 rows of 8192 bf16 with a residual to e4m3 in groups of 128: 194 us
+// (4.8 TB/s); one row of 4096: 4 us, a launch.
 
 #include <torch/extension.h>
 #include <ATen/DeviceGuard.h>

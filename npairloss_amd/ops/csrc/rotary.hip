@@ -11,6 +11,9 @@
 // uses it for all heads of q and k.  An item is eight pairs (two 16-byte
 // accesses in 16-bit types), or one pair where widths or addresses do not
 // allow that.
+//
+// 4 x 8192 tokens, 32 + 8 heads of 128 bf16: 123 us a direction (5.4 TB/s); 64 x 197 tokens, 12
+// heads of 64 fp16: 14.5 us (5.3 TB/s); 32 tokens: 4 us, a launch.
 
 #include <torch/extension.h>
 #include <ATen/DeviceGuard.h>
