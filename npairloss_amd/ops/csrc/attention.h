@@ -116,6 +116,10 @@ DEVINL const T* g_row(const AttnArgs& a, int b, int i, int h) {
 
 DEVINL float lane_of(float v, int lane) { return __shfl(v, lane, WAVE); }
 
+// Whether a row's sums, two of the width a lane, are NaN throughout: they stay so whatever
+// follows, and inputs that are NaN everywhere end their rows at once.
+DEVINL bool lost(const float (&x)[2], int lane, int D) { return __all((lane >= D || x[0] != x[0]) && (lane + 64 >= D || x[1] != x[1])); }
+
 // Widths up to 128: two elements a lane.
 template <typename T>
 DEVINL void forward_row(const AttnArgs& a, int b, int i, int h) {
@@ -151,6 +155,7 @@ DEVINL void forward_row(const AttnArgs& a, int b, int i, int h) {
       for (int x = 0; x < 2; ++x)
         if (lane + 64 * x < a.D) o[x] += w * to_f(v[lane + 64 * x]);
     }
+    if (total != total && lost(o, lane, a.D)) break;
   }
   const int64_t at_o = ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D;
   T* out = static_cast<T*>(a.o) + at_o;
@@ -190,6 +195,7 @@ DEVINL void dq_row(const AttnArgs& a, int b, int i, int h, float delta) {
       for (int x = 0; x < 2; ++x)
         if (lane + 64 * x < a.D) dq[x] += w * to_f(k[lane + 64 * x]);
     }
+    if (lost(dq, lane, a.D)) break;
   }
   T* out = static_cast<T*>(a.dq) + ((static_cast<int64_t>(b) * a.Lq + i) * a.H + h) * a.D;
 #pragma unroll
@@ -203,9 +209,10 @@ DEVINL void dkv_row(const AttnArgs& a, int b, int j, int c) {
   const T* k = k_row<T>(a, b, j, c);
   const T* v = v_row<T>(a, b, j, c);
   float dk[2] = {0.f, 0.f}, dv[2] = {0.f, 0.f};
-  for (int h = c * group; h < (c + 1) * group; ++h) {
+  bool all = false;
+  for (int h = c * group; h < (c + 1) * group && !all; ++h) {
     const float slope = a.slopes != nullptr ? a.slopes[h] : 0.f;
-    for (int i0 = 0; i0 < a.Lq; i0 += WAVE) {
+    for (int i0 = 0; i0 < a.Lq && !all; i0 += WAVE) {
       const int i = i0 + lane;
       const bool sees = i < a.Lq && row_sees<T>(a, b, i, j);
       float p = 0.f, ds = 0.f;
@@ -228,6 +235,7 @@ DEVINL void dkv_row(const AttnArgs& a, int b, int j, int c) {
             dv[x] += wp * to_f(g[lane + 64 * x]);
           }
       }
+      all = lost(dk, lane, a.D) && lost(dv, lane, a.D);
     }
   }
   const int64_t out = ((static_cast<int64_t>(b) * a.Lk + j) * a.Hk + c) * a.D;

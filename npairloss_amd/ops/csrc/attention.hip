@@ -161,9 +161,9 @@ std::vector<torch::Tensor> attention_fwd(torch::Tensor q, torch::Tensor k, torch
   a.o = o.data_ptr();
   a.lse = lse.data_ptr<float>();
   auto stream = at::hip::getCurrentHIPStream();
-  const bool tiled = attention_in_tiles(a);
-  const Ranges ranges(a, q_doc, k_doc, tiled, stream);
-  const auto order = tiled ? block_order(ranges.q, a.Lq, ranges.k, a.Lk, a.B, stream) : torch::Tensor();
+  const bool ordered = attention_in_tiles(a) && a.Lq > kBlockRows;
+  const Ranges ranges(a, q_doc, k_doc, ordered, stream);
+  const auto order = ordered ? block_order(ranges.q, a.Lq, ranges.k, a.Lk, a.B, stream) : torch::Tensor();
   a.q_order = order_of(order);
   DISPATCH_FLOAT(q.scalar_type(), "attention", [&] { attention_forward<T>(a, ranges_of(ranges.k), q.options(), stream); });
   HIP_CHECK_LAST();

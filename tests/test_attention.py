@@ -235,6 +235,19 @@ def test_not_finite_where_it_is_seen(device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [16, 80, 128])
+def test_nan_everywhere(D, dtype, device):
+    """NaN where anything is seen, zeros where nothing is."""
+    x = torch.full((1, 700, 2, D), math.nan, dtype=dtype, device=device)
+    ids = torch.zeros(1, 700, dtype=torch.int32, device=device)
+    ids[:, 650:] = -1
+    got = run(x, x, x, x, dict(documents=ids, causal=True))
+    for n, g in got.items():
+        assert g[:, :650].isnan().all() and (g[:, 650:] == 0).all(), n
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
 def test_strides(dtype, device):
     """Views of a packed projection, heads first, elements apart, rows off the border, a broadcast gradient."""
     g = torch.Generator().manual_seed(7)
