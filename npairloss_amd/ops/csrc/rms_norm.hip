@@ -16,8 +16,8 @@
 // not a multiple of eight elements take the same kernels with one element to
 // an access, neighbouring lanes on neighbouring elements.
 //
-// 12608 rows of 768 bf16 with a residual: 15.5 us forward (5.0 TB/s), 22.8 and 3.9 backward
-// (3.4 TB/s: a workgroup walks over rows to keep the weight's gradient in registers, and each
+// 12608 rows of 768 bf16 with a residual: 15.5 us forward (5.0 TB/s), 19.3 backward with the
+// weight's sums (4.0 TB/s: a workgroup walks over rows to keep the weight's gradient in registers, and each
 // waits for its row); 16384 rows of 8192 bf16 with a residual to e4m3 in groups of 128: 194 us
 // (4.8 TB/s); one row of 4096: 4 us, a launch.
 
@@ -395,8 +395,13 @@ std::vector<torch::Tensor> rms_norm_bwd(torch::Tensor dy, c10::optional<torch::T
       constexpr int TPR = decltype(tpr)::value, NCH = decltype(nch)::value;
       constexpr int kThreads = TPR > 256 ? TPR : 256;
       constexpr int kRows = kThreads / TPR;
-      // two workgroups a CU of 256 threads, one of 1024
-      const int64_t grid = std::min<int64_t>((N + kRows - 1) / kRows, TPR > 256 ? 256 : 512);
+      // Two workgroups a CU of 256 threads, one of 1024: each writes a row of sums, which are
+      // read again.  Four where 16-bit rows of few registers leave each three rows and more:
+      // bf16, two against four, us: 12608 rows of 768 23.5 : 19.3, 32768 of 512 29 : 23, 8192
+      // of 4096 79 : 58, but 8192 of 2048 27.5 : 30.9 and 12608 of 768 fp32 27.9 : 29.8.
+      const int64_t steps = (N + kRows - 1) / kRows;
+      const bool four = sizeof(T) == 2 && NCH <= 2 && steps >= 3 * 1024;
+      const int64_t grid = std::min<int64_t>(steps, TPR > 256 ? 256 : four ? 1024 : 512);
       auto part = torch::empty({grid, D}, s.options().dtype(at::kFloat));
       auto launch = [&](auto kernel) {
         kernel<<<grid, kThreads, 0, stream>>>(

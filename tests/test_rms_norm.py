@@ -68,6 +68,19 @@ def test_formula(shape, dtype, residual, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(13000, 24), (5000, 2500)])
+def test_weight_gradient_of_many_rows(shape, dtype, device):
+    """Summed over as many workgroups as there are: a wave adds up to 4 of 13000 rows or 10 of
+    5000, 3 joins follow, then up to 1024 partial sums 32 at a time (32 and 31 additions): 76."""
+    x, w, _, dy, _ = inputs(*shape, dtype, device, False)
+    got = torch.autograd.grad(rms_norm(x, w.requires_grad_(), eps=EPS), w, dy)[0]
+    _, _, dw, (_, _, nrm, dyf) = formula(x, w.detach(), dy)
+    total = (dyf * nrm).abs().sum(0)
+    assert_within(got, dw, dw.abs() * half_step(dtype) + total * (CHAIN + 76 * U) + least(dtype), "dweight")
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_gradient_against_differences(device):
     """<gradient, u> against central differences of the formula in 64 bits."""
     x, w, r, dy, ds = inputs(6, 40, torch.float32, device, True, seed=3)
