@@ -579,8 +579,9 @@ DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(-static_cast<float
 // tiles.
 //   P^T = 2^(S^T - lse), dS^T = P^T (V dO^T - delta) bend, dQ^T += K^T dS^T
 // A kernel of its own and not sums of dK's workgroups into dQ: those would have to be atomic,
-// in an order that changes, or another pass.  It costs two of seven products.  64 images of 197 tokens, 12 heads of 64 bf16: 47 us; 8191 tokens, 16 heads of
-// 128 fp16, causal: 460 us, 900 TFLOP/s, of 1087 in a large library product.
+// in an order that changes, or another pass.  It costs two of seven products.  64 images of
+// 197 tokens, 12 heads of 64 bf16: 47 us; 8191 tokens, 16 heads of 128 fp16, causal: 460 us,
+// 900 TFLOP/s, of 1087 in a large library product.
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
   constexpr int KT = sizeof(T) == 2 && DP == 64 ? 64 : 32;
