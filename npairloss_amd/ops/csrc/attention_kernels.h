@@ -582,7 +582,7 @@ DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(-static_cast<float
 // in an order that changes, or another pass.  It costs two of seven products.  64 images of
 // 197 tokens, 12 heads of 64 bf16: 47 us; 8191 tokens, 16 heads of 128 fp16, causal: 460 us,
 // 900 TFLOP/s, of 1087 in a large library product.
-template <typename T, int DP, Score SC>
+template <typename T, int DP, Score SC, bool FINE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
   constexpr int KT = sizeof(T) == 2 && DP == 64 ? 64 : 32;
   __shared__ __attribute__((aligned(16))) T ks[2][KT * DP];
@@ -681,14 +681,17 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   auto step = [&](bool masked, int j, auto buf) {
     const Reader<T, DP> at = reader.fresh();
     f32x16 s[kSub], dp[kSub];
-    Frag<T> ds[kSub][2];
+    Frag<T> ds[kSub][2], rest[FINE ? kSub : 1][2];
     auto score = [&](int n, int i, const Frag<T>& f) {
       if (i == 0) s[n] = zeros16(), dp[n] = zeros16();
       if (i % 2 == 0) product(f, qf[i / 2], s[n]);
       else product(f, gf[i / 2], dp[n]);
     };
     auto score_read = [&](int n, int i) { return at.rows(i % 2 == 0 ? ks[buf] : vs[buf], 32 * n, i / 2); };
-    auto output = [&](int n, int i, const Frag<T>& f) { product(f, ds[n][i / kWide], dq[i % kWide]); };
+    auto output = [&](int n, int i, const Frag<T>& f) {
+      product(f, ds[n][i / kWide], dq[i % kWide]);
+      if constexpr (FINE) product(f, rest[n][i / kWide], dq[i % kWide]);
+    };
     auto output_read = [&](int n, int i) { return at.columns(ks[buf], 32 * n + 16 * (i / kWide), i % kWide); };
     uint32_t bits[kSub];  // one body for all tiles, as for dK and dV
     auto mask = [&](int n) {
@@ -718,6 +721,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
         if (capped(SC)) x[y] *= bend;
       }
       ds[n][r / 8].set2(r % 8, x[0], x[1]);
+      if constexpr (FINE) rest[n][r / 8].set2(r % 8, x[0] - to_f(ds[n][r / 8].v[r % 8]), x[1] - to_f(ds[n][r / 8].v[r % 8 + 1]));
     };
     constexpr int kA = 2 * kSteps, kB = 2 * kWide;  // products of scores and of outputs
     if constexpr (kSub == 2 && DP == 64) {
@@ -807,7 +811,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
 // 197 tokens, 12 heads of 64 bf16: 53 us; 8191 tokens, 16 heads on 4 of 128 fp16, causal:
 // 790 us, 700 TFLOP/s, of 1087 in a large library product, and 60 us for the join of eight
 // parts (4.5 TB/s).
-template <typename T, int DP, Score SC>
+template <typename T, int DP, Score SC, bool FINE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_kernel(AttnArgs a, const DocRange* ranges, int k_blocks, int splits, float* __restrict__ part) {
   constexpr bool kHalf = sizeof(T) == 2 && DP == 128;
   constexpr int QT = sizeof(T) == 2 && DP == 64 ? 64 : 32, kKeys = 32 * kWaves;
@@ -916,7 +920,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
   auto step = [&](bool masked, int i0, float slope2, auto buf) {
     const Reader<T, DP> at = reader.fresh();
     f32x16 s[kSub], dp[kSub];
-    Frag<T> p[kSub][2], ds[kSub][2];
+    Frag<T> p[kSub][2], ds[kSub][2], left[FINE ? kSub : 1][2];
     auto score = [&](int n, int i, const Frag<T>& f) {
       if (i == 0) s[n] = zeros16(), dp[n] = zeros16();
       if (i % 2 == 0) product(f, kf[i / 2], s[n]);
@@ -926,6 +930,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
     auto output = [&](int n, int i, const Frag<T>& f) {
       if (i % 2 == 0) product(f, p[n][i / 2 / kWide], dv[i / 2 % kWide]);
       else product(f, ds[n][i / 2 / kWide], dk[i / 2 % kWide]);
+      if constexpr (FINE)
+        if (i % 2 == 1) product(f, left[n][i / 2 / kWide], dk[i / 2 % kWide]);
     };
     auto output_read = [&](int n, int i) { return at.columns(i % 2 == 0 ? (buf == 0 ? gs0 : gs1) : (buf == 0 ? qs0 : qs1), 32 * n + 16 * (i / 2 / kWide), i / 2 % kWide); };
     // One body for all tiles: bodies that differ by their masks would each keep the sums
@@ -969,6 +975,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
       }
       p[n][r / 8].set2(r % 8, w[0], w[1]);
       ds[n][r / 8].set2(r % 8, g[0], g[1]);
+      if constexpr (FINE) left[n][r / 8].set2(r % 8, g[0] - to_f(ds[n][r / 8].v[r % 8]), g[1] - to_f(ds[n][r / 8].v[r % 8 + 1]));
     };
     constexpr int kA = 2 * kSteps, kB = 4 * kWide;  // products of scores and of outputs: as many
     static_assert(kA == kB && 16 % kA == 0, "pairs of registers go by products");
@@ -1171,7 +1178,7 @@ void run_forward(const AttnArgs& a, const DocRange* ranges, const torch::TensorO
 template <typename T, int DP, Score SC>
 void run_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q_ranges, const torch::TensorOptions& options, hipStream_t stream) {
   const int q_tiles = (a.Lq + kQueries - 1) / kQueries, k_blocks = (a.Lk + kQueries - 1) / kQueries;
-  dq_tiles_kernel<T, DP, SC><<<blocks_for(static_cast<int64_t>(a.B) * a.H * q_tiles, 1), kThreads, 0, stream>>>(a, k_ranges, q_tiles);
+  const int64_t q_grid = blocks_for(static_cast<int64_t>(a.B) * a.H * q_tiles, 1);
   // Blocks of keys that do not fill the chip four times over are split over heads and
   // queries, down to eight tiles of queries, for their sums to be joined: a causal mask makes
   // their lengths uneven, and heads that share keys make them few.  Split in four where
@@ -1185,7 +1192,19 @@ void run_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q
   torch::Tensor part;
   if (splits > 1) part = torch::empty({splits, 2, rows, a.D}, options.dtype(at::kFloat));
   float* p = splits > 1 ? part.data_ptr<float>() : nullptr;
-  dkv_tiles_kernel<T, DP, SC><<<blocks_for(base * splits, 1), kThreads, 0, stream>>>(a, q_ranges, k_blocks, splits, p);
+  auto launch = [&](auto fine) {
+    dq_tiles_kernel<T, DP, SC, decltype(fine)::value><<<q_grid, kThreads, 0, stream>>>(a, k_ranges, q_tiles);
+    dkv_tiles_kernel<T, DP, SC, decltype(fine)::value><<<blocks_for(base * splits, 1), kThreads, 0, stream>>>(a, q_ranges, k_blocks, splits, p);
+  };
+  // fp16 score gradients of small calls are multiplied twice, once for what rounding took from
+  // them: over few scores it was up to 1.55 times as much as the result's own rounding leaves (1.2
+  // with the second product), and such calls are as long as their launches: 23 rows of 3
+  // tokens, 6 heads of 32, forward and backward 25.1 us with it, where bf16, which has neither it
+  // nor scaled gradients, takes 20.8; 256 tokens, 16 heads of 128 64 and 57.
+  bool done = false;
+  if constexpr (std::is_same<T, fp16_t>::value)
+    if (static_cast<int64_t>(a.B) * a.H * a.Lq * a.Lk <= 1 << 20) launch(std::true_type()), done = true;
+  if (!done) launch(std::false_type());
   if (splits > 1) join_dkv_kernel<T><<<blocks_for(rows, kWaves), kThreads, 0, stream>>>(a, splits, rows, p);
 }
 

@@ -161,6 +161,26 @@ def test_formula(name, dtype, device):
         assert torch.equal(attention(q, k, v, **more), got["out"])
 
 
+LARGER = {
+    "plain": case(B=1, Lq=520, H=4, D=64),
+    "causal, prefix, slopes": case(B=1, Lq=520, H=4, Hk=2, D=128, causal=True, prefix=[70], slopes=True),
+    "documents, capped": case(B=1, Lq=530, H=4, D=64, documents="packed", softcap=20.0),
+    "documents, capped, slopes": case(B=1, Lq=520, H=4, Hk=1, D=128, documents="mixed", softcap=20.0, slopes=True),
+}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", LARGER)
+def test_formula_of_larger_calls(name, dtype, device):
+    """Over 2^20 scores: fp16 score gradients are multiplied once."""
+    q, k, v, dout, more = inputs(LARGER[name], dtype, device)
+    got = run(q, k, v, dout, more)
+    want, tol = exact(q, k, v, dout, more, dtype)
+    for n in want:
+        assert_within(got[n], want[n], tol[n], n)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("name", ["capped", "documents, causal", "causal, more keys"])
 def test_gradient_against_differences(name, device):
