@@ -273,8 +273,8 @@ class Trainer:
                     f"training diverged: loss={lv} at iter {self.iter}")
         # detach EVERYTHING: a non-detached Function output held across a
         # later hipGraph capture keeps the autograd node (and its stream
-        # state) alive and hipGraphInstantiate segfaults (bisect: tools/
-        # debug_capture.py — hold-the-stats-dict was the exact trigger)
+        # state) alive and hipGraphInstantiate segfaults (a held stats dict
+        # was the exact trigger)
         return {
             "loss": out.loss.detach(), "top1": out.retrieve_top1.detach(),
             "top5": out.retrieve_top5.detach(), "top10": out.retrieve_top10.detach(),
@@ -358,8 +358,8 @@ class Trainer:
         out = g["out"]
         # detach EVERYTHING: a non-detached Function output held across a
         # later hipGraph capture keeps the autograd node (and its stream
-        # state) alive and hipGraphInstantiate segfaults (bisect: tools/
-        # debug_capture.py — hold-the-stats-dict was the exact trigger)
+        # state) alive and hipGraphInstantiate segfaults (a held stats dict
+        # was the exact trigger)
         return {
             "loss": out.loss.detach(), "top1": out.retrieve_top1.detach(),
             "top5": out.retrieve_top5.detach(), "top10": out.retrieve_top10.detach(),
