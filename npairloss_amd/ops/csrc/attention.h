@@ -36,7 +36,10 @@ struct AttnArgs {
   // backward
   const void* dout; RowStrides gs;
   float* delta;          // [B, H, Lq]: sum_d dout o
-  unsigned* grad_top;    // bits of the largest |dout| (fp16) or null
+  // fp16, or null
+  float* row_top;        // [B, H, Lq]: the largest finite |dout| of a query
+  float* block_top;      // [B, H, blocks of 32 queries]: the largest of those
+  float* key_lift;       // [B, Hk, Lk]: what a key's score gradients are multiplied by
   void* dq;              // [B, Lq, H, D]
   void* dk; void* dv;    // [B, Lk, Hk, D]
 };
@@ -85,6 +88,14 @@ DEVINL float transformed(const AttnArgs& a, float dot, float slope, int distance
   if (a.softcap > 0.f) s = cap<T>(s / a.softcap, a.softcap, *bend);
   return (s - slope * static_cast<float>(distance)) * kLog2e;
 }
+
+// fp16 has 2^-14 for its least normal number, and over long rows weights and score
+// gradients lie under it.  Weights are taken times 2^10 in the products over
+// queries; score gradients times a power of two that brings the largest |dO| (of the
+// query for dQ, of all queries that see the key for dK) to 1/4 .. 1/2, so that they
+// overflow only where a sum over the width is over 2^17 times that (dK's, which have the
+// weights' 2^10 as well, 2^7 times), and then the row is done again.
+DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(-static_cast<float>(ilogbf(top)) - 2.f) : 1.f; }
 
 // --- one row with one wave: any mask, and nothing that a masked key holds ---
 

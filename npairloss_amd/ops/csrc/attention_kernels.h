@@ -568,13 +568,6 @@ __global__ __launch_bounds__(kThreads) void join_splits_kernel(AttnArgs a, int s
 
 // --- backward ---------------------------------------------------------------
 
-// fp16 has 2^-14 for its least normal number, and over long rows weights and score
-// gradients lie under it.  Weights are taken times 2^10 in the products over
-// queries; score gradients times a power of two that brings the largest |dO| (of the
-// query for dQ, of all for dK) to 1/4 .. 1/2, so that they overflow only where a sum
-// over the width is over 2^17 times that, and then the row is done again.
-DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(-static_cast<float>(ilogbf(top)) - 2.f) : 1.f; }
-
 // dQ of 32 queries a wave, and delta for both: lanes are queries, K and V pass by in
 // tiles.
 //   P^T = 2^(S^T - lse), dS^T = P^T (V dO^T - delta) bend, dQ^T += K^T dS^T
@@ -628,10 +621,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
   // dS of fp16 is scaled into its range (see grad_scale), through the exponent
   float lift = 1.f;
   if constexpr (std::is_same<T, fp16_t>::value) {
-    lift = grad_scale(fmaxf(high, other_half(high)));
-    high = wave_reduce_max(high);  // a maximum does not depend on the order it is taken in
-    if (lane == 0 && __float_as_uint(high) > __hip_atomic_load(a.grad_top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-      atomicMax(a.grad_top, __float_as_uint(high));
+    high = fmaxf(high, other_half(high));
+    lift = grad_scale(high);
+    if (ok && lane < 32) a.row_top[bh * a.Lq + i] = high;
+    high = wave_reduce_max(high);
+    if (lane == 0 && ok) a.block_top[bh * ((a.Lq + 31) / 32) + i / 32] = high;
   }
   const float lse = ok ? a.lse[bh * a.Lq + i] - log2f(lift) : INFINITY;
   // rows that are not there decide nothing, and nothing of them is kept
@@ -907,7 +901,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
   };
   constexpr float kWeightLift = sizeof(T) == 2 && std::is_same<T, fp16_t>::value ? 10.f : 0.f;  // see grad_scale
   float lift = 1.f;
-  if constexpr (std::is_same<T, fp16_t>::value) lift = grad_scale(__uint_as_float(*a.grad_top));
+  if constexpr (std::is_same<T, fp16_t>::value) lift = in ? a.key_lift[bc * a.Lk + j] : 1.f;
   const int* d0 = a.q_doc != nullptr ? a.q_doc + static_cast<int64_t>(b) * a.Lq : nullptr;
 
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -1194,6 +1188,7 @@ void run_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q
   float* p = splits > 1 ? part.data_ptr<float>() : nullptr;
   auto launch = [&](auto fine) {
     dq_tiles_kernel<T, DP, SC, decltype(fine)::value><<<q_grid, kThreads, 0, stream>>>(a, k_ranges, q_tiles);
+    if constexpr (std::is_same<T, fp16_t>::value) key_lifts(a, q_ranges, stream);
     dkv_tiles_kernel<T, DP, SC, decltype(fine)::value><<<blocks_for(base * splits, 1), kThreads, 0, stream>>>(a, q_ranges, k_blocks, splits, p);
   };
   // fp16 score gradients of small calls are multiplied twice, once for what rounding took from

@@ -20,7 +20,10 @@ inline bool attention_in_tiles(const AttnArgs& a) {
 template <typename T>
 void attention_forward(const AttnArgs& a, const DocRange* ranges, const torch::TensorOptions& options, hipStream_t stream);
 
-// `a.delta` (and `a.grad_top`, zeroed, for fp16) are written here.
+// `a.key_lift` from `a.row_top` and `a.block_top`.
+void key_lifts(const AttnArgs& a, const DocRange* q_ranges, hipStream_t stream);
+
+// `a.delta` (and for fp16 `a.row_top`, `a.block_top` and `a.key_lift`) are written here.
 template <typename T>
 void attention_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q_ranges, const torch::TensorOptions& options,
                         hipStream_t stream);

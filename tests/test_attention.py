@@ -429,3 +429,28 @@ def test_repeated_and_on_another_stream():
         again = run(q, k, v, dout, more)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["causal, more keys", "documents", "documents, mixed", "documents, causal", "prefix", "uneven", "long"])
+def test_large_gradients_that_nobody_sees(name, dtype, device):
+    """Gradient rows of 6e4 beside ones of 1e-3, in other documents, in padding, in another batch
+    row and at earlier places: keys that see none of them get dK and dV as if they held zeros, bit
+    for bit, as what is added for them is zero."""
+    c = CASES[name] if name in CASES else case(B=2, Lq=1500, H=2, Hk=1, D=64, documents="packed")
+    q, k, v, dout, more = inputs(c, dtype, device)
+    B, Lq, Lk = q.shape[0], q.shape[1], k.shape[1]
+    seen = mask_of(more, B, Lq, Lk)[0].expand(B, 1, Lq, Lk)[:, 0]
+    large = torch.zeros(B, Lq, dtype=torch.bool)
+    large[1:] = True
+    if more.get("documents") is not None:
+        large |= (more["documents"].cpu() < 0) | (more["documents"].cpu() == 1)
+    else:
+        large[:, :Lq // 2] = True
+    beside = lambda x: torch.where(large[..., None, None].to(device), x, dout * 1e-3)  # noqa: E731
+    got, want = run(q, k, v, beside(dout.sign() * 6e4), more), run(q, k, v, beside(torch.zeros_like(dout)), more)
+    fine = ~(seen & large[..., None]).any(1) & seen.any(1)
+    assert fine.any()
+    for n in ("dk", "dv"):
+        assert torch.equal(got[n][fine.to(device)], want[n][fine.to(device)]), n
