@@ -10,7 +10,7 @@
 #include <vector>
 
 std::vector<torch::Tensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> residual,
-                                        double eps, int64_t group);
+                                        double eps, int64_t group, at::IntArrayRef shape);
 std::vector<torch::Tensor> rms_norm_bwd(torch::Tensor dy, c10::optional<torch::Tensor> dsum, torch::Tensor s,
                                         torch::Tensor weight, torch::Tensor inv);
 std::vector<torch::Tensor> rotary_turn(torch::Tensor q, c10::optional<torch::Tensor> k, torch::Tensor positions,
@@ -80,9 +80,10 @@ void check_norm(const Tensor& x, const Tensor& weight, const OptTensor& residual
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps) {
     const Tensor w = weight.contiguous();
-    auto got = rms_norm_fwd(rows(x), w, residual.has_value() ? OptTensor(rows(*residual)) : c10::nullopt, eps, -1);
-    variable_list out{shaped(got[0], x.sizes())};
-    if (residual.has_value()) out.push_back(shaped(got[2], x.sizes()));
+    // made in their shape: a view from within a function may not be changed in place
+    auto got = rms_norm_fwd(rows(x), w, residual.has_value() ? OptTensor(rows(*residual)) : c10::nullopt, eps, -1, x.sizes());
+    variable_list out{got[0]};
+    if (residual.has_value()) out.push_back(got[2]);
     ctx->save_for_backward({residual.has_value() ? out[1] : x, w, got[1]});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->set_materialize_grads(false);
@@ -154,8 +155,8 @@ struct Attention : torch::autograd::Function<Attention> {
       ctx->saved_data["causal"] = causal;
       ctx->saved_data["own"] = own;
     }
-    // saved as it lies, given out as a view of its own, so that the node does not hold itself
-    return own == width ? got[0].view(got[0].sizes()) : got[0].narrow(3, 0, own);
+    // not a view, which from within a function may not be changed in place
+    return own == width ? got[0] : got[0].narrow(3, 0, own).contiguous();
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -190,11 +191,9 @@ std::vector<Tensor> rms_norm_fp8(Tensor x, Tensor weight, OptTensor residual, do
   // groups want eight neighbours to a lane: rows that begin off a 16-byte border are copied
   auto placed = [&](const Tensor& t) { return group > 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0 ? t.clone() : t; };
   auto got = rms_norm_fwd(placed(rows(x)), placed(weight.contiguous()), residual.has_value() ? OptTensor(placed(rows(*residual))) : c10::nullopt,
-                          eps, group);
+                          eps, group, x.sizes());
   if (x.dim() != 2) {
     auto sizes = x.sizes().vec();
-    got[0] = got[0].view(sizes);
-    if (residual.has_value()) got[2] = got[2].view(sizes);
     sizes.back() = got[1].size(1);
     got[1] = got[1].view(sizes);
   }

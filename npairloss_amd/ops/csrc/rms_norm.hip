@@ -24,6 +24,7 @@
 #include <torch/extension.h>
 #include <ATen/DeviceGuard.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/util/accumulate.h>
 
 #include "vec.h"
 
@@ -323,22 +324,24 @@ void check_like(const torch::Tensor& x, const c10::optional<torch::Tensor>& r) {
 
 }  // namespace
 
-// {y or codes, scales (e4m3) or inv, sum (if there is a residual)}.  `group` < 0:
-// y in x's type; 0: e4m3 with a scale a row; > 0: with a scale for every group.
+// {y or codes, scales (e4m3) or inv, sum (if there is a residual)}, y, codes and sum in
+// `shape`.  `group` < 0: y in x's type; 0: e4m3 with a scale a row; > 0: with a scale for
+// every group.
 std::vector<torch::Tensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight,
                                         c10::optional<torch::Tensor> residual, double eps,
-                                        int64_t group) {
+                                        int64_t group, at::IntArrayRef shape) {
   check_rows(x, weight);
   check_like(x, residual);
+  TORCH_CHECK(c10::multiply_integers(shape) == x.numel(), "rms_norm: rows and shape differ");
   const int64_t N = x.size(0), D = x.size(1);
   const bool fp8 = group >= 0;
   TORCH_CHECK(group <= 0 || ((group & (group - 1)) == 0 && group >= 16 && group <= 512 && D % group == 0),
               "rms_norm: a group is a power of two from 16 to 512 that divides the row");
   at::DeviceGuard guard(x.device());
-  auto y = fp8 ? torch::empty({N, D}, x.options().dtype(at::kFloat8_e4m3fn)) : torch::empty_like(x);
+  auto y = torch::empty(shape, fp8 ? x.options().dtype(at::kFloat8_e4m3fn) : x.options());
   auto second = fp8 ? torch::empty({N, group > 0 ? D / group : 1}, x.options().dtype(at::kFloat))
                     : torch::empty({N}, x.options().dtype(at::kFloat));
-  torch::Tensor sum = residual.has_value() ? torch::empty_like(x) : torch::Tensor();
+  torch::Tensor sum = residual.has_value() ? torch::empty(shape, x.options()) : torch::Tensor();
   std::vector<torch::Tensor> out{y, second};
   if (residual.has_value()) out.push_back(sum);
   if (N == 0) return out;

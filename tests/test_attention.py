@@ -454,3 +454,25 @@ def test_large_gradients_that_nobody_sees(name, dtype, device):
     assert fine.any()
     for n in ("dk", "dv"):
         assert torch.equal(got[n][fine.to(device)], want[n][fine.to(device)]), n
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [16, 20, 128])
+def test_an_output_changed_in_place(D, device):
+    """It may be; a backward pass that has lost what it needs by that says so, and is never wrong."""
+    q, k, v, dout, more = inputs(case(Lq=6, H=2, D=D), torch.float32, device)
+    want = run(q, k, v, dout, more)
+    q.requires_grad_()
+    o = attention(q, k, v)
+    o *= 2
+    assert torch.equal(o.detach(), want["out"] * 2)
+    try:
+        o.backward(dout / 2)
+    except RuntimeError as e:
+        assert "modified by an inplace operation" in str(e)
+    else:
+        assert torch.equal(q.grad, want["dq"])
+    with torch.no_grad():
+        o = attention(q, k, v)
+        o *= 2
+    assert torch.equal(o, want["out"] * 2)

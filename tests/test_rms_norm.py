@@ -253,3 +253,24 @@ def test_captured():
     for out in replays(train):
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", [(16,), (6, 16), (2, 3, 16)])
+def test_outputs_changed_in_place(shape, device):
+    """y is not kept for the backward pass and may be changed; the sum is, which then says so."""
+    g = torch.Generator().manual_seed(0)
+    x, r = (torch.randn(*shape, generator=g).to(device) for _ in range(2))
+    w = torch.ones(16, device=device, requires_grad=True)
+    want = rms_norm(x, w)
+    (grad,) = torch.autograd.grad(want, w, x)
+    y = rms_norm(x, w)
+    y *= 2
+    assert torch.equal(y.detach(), want.detach() * 2)
+    y.backward(x / 2)
+    assert torch.equal(w.grad, grad)
+    y, s = rms_norm(x, w, r)
+    s += 1
+    assert torch.equal(s.detach(), x + r + 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(x)
