@@ -133,7 +133,11 @@ struct Rotary : torch::autograd::Function<Rotary> {
 // Rows as the attention kernels read them: `width` wide (zeros behind), 16-byte
 // borders, under 16 MB apart (offsets within a tile are 32 bits).
 Tensor ready(const Tensor& x, int64_t width) {
-  if (x.size(3) != width) return at::constant_pad_nd(x, {0, width - x.size(3)});
+  if (x.size(3) != width) {  // not torch's padding, which keeps an order of dimensions where it knows one
+    Tensor out = at::zeros({x.size(0), x.size(1), x.size(2), width}, x.options());
+    out.narrow(3, 0, x.size(3)).copy_(x);
+    return out;
+  }
   const int64_t size = x.element_size(), per16 = 16 / size;
   const bool fits = x.stride(3) == 1 && x.stride(0) % per16 == 0 && x.stride(1) % per16 == 0 && x.stride(2) % per16 == 0 &&
                     reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && (x.size(1) <= 1 || x.stride(1) * size <= (1 << 24));

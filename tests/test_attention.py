@@ -476,3 +476,18 @@ def test_an_output_changed_in_place(D, device):
         o = attention(q, k, v)
         o *= 2
     assert torch.equal(o, want["out"] * 2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L,D", [(50, 1), (50, 20), (50, 32), (1, 20)])
+def test_lengths_innermost(L, D, dtype, device):
+    """A feature map [batch, heads, width, pixels] taken as [batch, pixels, heads, width], inputs or
+    the gradient, at widths that are padded and one that is not."""
+    g = torch.Generator().manual_seed(7)
+    inputs = [torch.randn(2, L, h, D, generator=g).to(dtype).to(device) for h in (4, 2, 2, 4)]
+    base = run(*inputs, dict(causal=True))
+    pixels = lambda x: x.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)  # noqa: E731
+    for turned in ((0, 1, 2), (3,), (0, 1, 2, 3)):
+        got = run(*(pixels(x) if n in turned else x for n, x in enumerate(inputs)), dict(causal=True))
+        assert all(torch.equal(got[n], base[n]) for n in base)
