@@ -92,10 +92,11 @@ DEVINL float transformed(const AttnArgs& a, float dot, float slope, int distance
 // fp16 has 2^-14 for its least normal number, and over long rows weights and score
 // gradients lie under it.  Weights are taken times 2^10 in the products over
 // queries; score gradients times a power of two that brings the largest |dO| (of the
-// query for dQ, of all queries that see the key for dK) to 1/4 .. 1/2, so that they
-// overflow only where a sum over the width is over 2^17 times that (dK's, which have the
-// weights' 2^10 as well, 2^7 times), and then the row is done again.
-DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(-static_cast<float>(ilogbf(top)) - 2.f) : 1.f; }
+// query for dQ, of all queries that see the key for dK) to 8 .. 16.  They overflow only
+// where weight times sum over the width is 2^12 times the largest |dO|, and then the row
+// is done again.  Lower, long rows lose bits: of 32768 even weights dQ was 3.0 times as far
+// off as by the result's own rounding with 1/4 .. 1/2, 1.4 times from 4 .. 8 on.
+DEVINL float grad_scale(float top) { return top > 0.f ? exp2f(3.f - static_cast<float>(ilogbf(top))) : 1.f; }
 
 // --- one row with one wave: any mask, and nothing that a masked key holds ---
 

@@ -901,7 +901,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_ke
   };
   constexpr float kWeightLift = sizeof(T) == 2 && std::is_same<T, fp16_t>::value ? 10.f : 0.f;  // see grad_scale
   float lift = 1.f;
-  if constexpr (std::is_same<T, fp16_t>::value) lift = in ? a.key_lift[bc * a.Lk + j] : 1.f;
+  if constexpr (std::is_same<T, fp16_t>::value) lift = in ? a.key_lift[bc * a.Lk + j] * exp2f(-kWeightLift) : 1.f;  // the weights in dS bring theirs
   const int* d0 = a.q_doc != nullptr ? a.q_doc + static_cast<int64_t>(b) * a.Lq : nullptr;
 
   f32x16 dk[DP / 32], dv[DP / 32];

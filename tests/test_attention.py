@@ -491,3 +491,30 @@ def test_lengths_innermost(L, D, dtype, device):
     for turned in ((0, 1, 2), (3,), (0, 1, 2, 3)):
         got = run(*(pixels(x) if n in turned else x for n, x in enumerate(inputs)), dict(causal=True))
         assert all(torch.equal(got[n], base[n]) for n in base)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("big", [50.0, 3000.0])
+def test_large_values(big, device):
+    """fp16 with values of tens, whose score gradients fit, and of thousands, whose may not: weights
+    near one by scores of four times the usual."""
+    q, k, v, dout, more = inputs(case(B=1, Lq=300, H=2, D=128, causal=True), torch.float16, device)
+    args = (q * 2, k * 2, v * big, dout, more)
+    got, (want, tol) = run(*args), exact(*args, torch.float16)
+    for n in want:
+        assert_within(got[n], want[n], tol[n], n)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_long_even_rows(dtype, device):
+    """Weights near 2^-15.  Each is rounded once, and so is each score gradient, by independent
+    parts of themselves: their sums are as far off, in the mean square, as the result's own
+    rounding leaves it.  Together that is sqrt(2) of it; 1.6 for means of 8192 results, whose
+    scatter is some hundredths."""
+    q, k, v, dout, more = inputs(case(B=1, Lq=64, Lk=32768, H=2, D=64), dtype, device)
+    args = (q * 0.1, k, v, dout, more)
+    got, (want, _) = run(*args), exact(*args, dtype)
+    off = lambda x, n: float((x.double().cpu() - want[n]).square().mean().sqrt())  # noqa: E731
+    for n in ("out", "dq"):
+        assert off(got[n], n) <= 1.6 * off(want[n].to(dtype), n), n
