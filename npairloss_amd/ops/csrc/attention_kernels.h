@@ -113,12 +113,20 @@ template <typename T, int DP, int NS>
 struct Online {
   f32x16 o[DP / 32];
   float top, l;
+  bool by_id;  // with documents: whether this half has seen a key
 
   DEVINL void clear() {
 #pragma unroll
     for (int x = 0; x < DP / 32; ++x) o[x] = zeros16();
     top = -INFINITY;
     l = 0.f;
+    by_id = false;
+  }
+
+  // Whether the query sees any key: its scores may all be -infinity, which is no reason for zeros.
+  DEVINL bool sees(const AttnArgs& a, const Query& q) const {
+    const bool other = __shfl_xor(static_cast<int>(by_id), 32, WAVE) != 0;
+    return a.k_doc == nullptr ? q.end > 0 : by_id || other;
   }
 
   template <Score SC>
@@ -158,9 +166,14 @@ struct Online {
       for (int n = 0; n < NS; ++n) {
         Seen<decltype(which)::value, false> seen(q.end - first - 32 * n, q.doc, kd + 32 * n);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] = seen(r) ? s[n][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) {
+          const bool ok = seen(r);
+          s[n][r] = ok ? s[n][r] : -INFINITY;
+          if (decltype(which)::value == kIds) by_id = by_id || ok;
+        }
       }
     };
+    if (mask == kSeen) by_id = true;
     if (mask == kEnds) apply(std::integral_constant<Mask, kEnds>());
     if (mask == kIds) apply(std::integral_constant<Mask, kIds>());
 #pragma unroll
@@ -368,7 +381,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
   }
 
   const float total = run.l + other_half(run.l);
-  const bool none = run.top == -INFINITY && !(total != total);
+  const bool none = !run.sees(a, q);
   uint32_t again = 0;
   if (repairs<T>(a)) again = bad_columns(ok && (!finite_column(run.o) || !(fabsf(total) <= FLT_MAX)));
   if (ok && !(again >> (lane % 32) & 1)) {
@@ -381,12 +394,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) 
   for (; again != 0; again &= again - 1) forward_row<T>(a, b, i0 + 32 * wave + __builtin_ctz(again), h);
 }
 
+// In place of the sum of weights, which is not negative, of a part in which a row sees no key.
+constexpr float kSeesNone = -1.f;
+
 // One row's joined sums (two of the width a lane), by one wave: the quotient, or
 // the row again where it is not finite.
 template <typename T>
-DEVINL void finish_row(const AttnArgs& a, int b, int i, int h, float o0, float o1, float top, float total) {
+DEVINL void finish_row(const AttnArgs& a, int b, int i, int h, float o0, float o1, float top, float total, bool none) {
   const int lane = threadIdx.x % WAVE;
-  const bool none = top == -INFINITY && !(total != total);
   if (repairs<T>(a) && __any(!(fabsf(o0) <= FLT_MAX && fabsf(o1) <= FLT_MAX && fabsf(total) <= FLT_MAX))) {
     forward_row<T>(a, b, i, h);
     return;
@@ -507,7 +522,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_spli
     j = following;
   }
 
-  const float total = run.l + other_half(run.l);
+  const float sum_here = run.l + other_half(run.l);
+  const float total = run.sees(a, q) ? sum_here : kSeesNone;
   if (lane < 32) tops[wave][lane] = run.top, totals[wave][lane] = total;
   __syncthreads();  // all tiles are used: their memory takes the sums
   float* join = reinterpret_cast<float*>(shared);
@@ -522,21 +538,22 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void forward_spli
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w][c]);
     float sum = 0.f, o0 = 0.f, o1 = 0.f;
+    bool none = true;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const float keep = tops[w][c] == -INFINITY && top != -INFINITY ? 0.f : tops[w][c] == top ? 1.f : __builtin_amdgcn_exp2f(tops[w][c] - top);
-      sum += keep * totals[w][c];
+      if (totals[w][c] != kSeesNone) none = false, sum += keep * totals[w][c];
       o0 += keep * join[(w * 32 + c) * kPad + lane % DP];
       if (DP > 64) o1 += keep * join[(w * 32 + c) * kPad + 64 + lane];
     }
     const int which = row0 + c;
     if (splits == 1) {
-      finish_row<T>(a, b, which % a.Lq, kv * group + which / a.Lq, o0, o1, top, sum);
+      finish_row<T>(a, b, which % a.Lq, kv * group + which / a.Lq, o0, o1, top, sum, none);
     } else {
       const int64_t to = ((static_cast<int64_t>(split) * a.B + b) * a.Hk + kv) * rows + which;
       part[to * DP + lane] = o0;
       if (DP > 64) part[to * DP + 64 + lane] = o1;
-      if (lane == 0) stats[to] = make_float2(top, sum);
+      if (lane == 0) stats[to] = make_float2(top, none ? kSeesNone : sum);
     }
   }
 }
@@ -548,12 +565,13 @@ __global__ __launch_bounds__(kThreads) void join_splits_kernel(AttnArgs a, int s
   const int lane = threadIdx.x % WAVE;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / WAVE;
   if (at >= count) return;
-  const float2 own = lane < splits ? stats[lane * count + at] : make_float2(-INFINITY, 0.f);
+  const float2 own = lane < splits ? stats[lane * count + at] : make_float2(-INFINITY, kSeesNone);
   float top = own.x;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, WAVE));
   const float keep = own.x == -INFINITY && top != -INFINITY ? 0.f : own.x == top ? 1.f : __builtin_amdgcn_exp2f(own.x - top);
-  const float sum = wave_reduce_sum(keep * own.y);
+  const bool none = __all(own.y == kSeesNone);
+  const float sum = wave_reduce_sum(own.y == kSeesNone ? 0.f : keep * own.y);
   float o0 = 0.f, o1 = 0.f;
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
@@ -563,7 +581,7 @@ __global__ __launch_bounds__(kThreads) void join_splits_kernel(AttnArgs a, int s
   }
   const int rows = a.H / a.Hk * a.Lq, row = at % rows;
   const int64_t bc = at / rows;
-  finish_row<T>(a, bc / a.Hk, row % a.Lq, bc % a.Hk * (a.H / a.Hk) + row / a.Lq, o0, o1, top, sum);
+  finish_row<T>(a, bc / a.Hk, row % a.Lq, bc % a.Hk * (a.H / a.Hk) + row / a.Lq, o0, o1, top, sum, none);
 }
 
 // --- backward ---------------------------------------------------------------

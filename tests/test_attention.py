@@ -518,3 +518,31 @@ def test_long_even_rows(dtype, device):
     off = lambda x, n: float((x.double().cpu() - want[n]).square().mean().sqrt())  # noqa: E731
     for n in ("out", "dq"):
         assert off(got[n], n) <= 1.6 * off(want[n].to(dtype), n), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["plain", "causal", "documents", "documents, mixed", "documents, causal", "few queries, long", "documents, one query", "in parts"])
+def test_scores_of_minus_infinity(name, dtype):
+    """Keys whose scores are -infinity for every query: where nothing else is seen weights are 0 / 0,
+    NaN in outputs and gradients, and where nothing is seen at all zeros, as on the CPU.  Behind a
+    cap c such a score is -c, and nothing is NaN."""
+    c = CASES[name] if name in CASES else case(B=2, Lq=2, Lk=1100, H=4, Hk=2, D=64)
+    got = {}
+    for device in ("cpu", "cuda"):
+        q, k, v, dout, more = inputs(c, dtype, device)
+        q[..., 0] = q[..., 0].abs() + 1
+        kd = more.get("key_documents", more.get("documents"))
+        bad = torch.zeros(k.shape[:2], dtype=torch.bool, device=device)
+        if kd is None:
+            bad[0] = True
+        elif "key_documents" in more:
+            bad[4] = True
+        else:
+            bad = kd == 1
+        k[..., 0] = torch.where(bad[..., None], -math.inf, k[..., 0].float()).to(dtype)
+        got[device] = run(q, k, v, dout, more)
+    assert got["cpu"]["out"].isnan().any() == (not c["softcap"]) and not got["cpu"]["out"].isnan().all()
+    for n, x in got["cpu"].items():
+        assert torch.equal(x.isnan(), got["cuda"][n].isnan().cpu()), n
+        assert n != "out" or torch.equal(x == 0, got["cuda"][n].cpu() == 0)
