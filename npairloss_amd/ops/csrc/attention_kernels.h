@@ -1209,14 +1209,15 @@ void run_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q
     if constexpr (std::is_same<T, fp16_t>::value) key_lifts(a, q_ranges, stream);
     dkv_tiles_kernel<T, DP, SC, decltype(fine)::value><<<blocks_for(base * splits, 1), kThreads, 0, stream>>>(a, q_ranges, k_blocks, splits, p);
   };
-  // fp16 score gradients of small calls are multiplied twice, once for what rounding took from
-  // them: over few scores it was up to 1.55 times as much as the result's own rounding leaves (1.2
-  // with the second product), and such calls are as long as their launches: 23 rows of 3
-  // tokens, 6 heads of 32, forward and backward 25.1 us with it, where bf16, which has neither it
-  // nor scaled gradients, takes 20.8; 256 tokens, 16 heads of 128 64 and 57.
+  // fp16 score gradients of rows of one tile are multiplied twice, once for what rounding took
+  // from them.  Without it dQ and dK are the further off the fewer keys a row has: 1.50 times
+  // as far as by the result's own rounding with 2 to 4, 1.45 with 16, 1.42 from 64 on; with it
+  // 1.15 and less.  It costs more where products are the longer part, which rows of one tile,
+  // loaded for 128 queries and keys, do not have: 64 rows of 32 tokens, 12 heads of 64, dQ and
+  // dK, dV 16.0 + 15.2 us, in bf16, with one product and no scaled gradients, 13.6 + 13.5.
   bool done = false;
   if constexpr (std::is_same<T, fp16_t>::value)
-    if (static_cast<int64_t>(a.B) * a.H * a.Lq * a.Lk <= 1 << 20) launch(std::true_type()), done = true;
+    if (a.Lq <= 32 && a.Lk <= 32) launch(std::true_type()), done = true;
   if (!done) launch(std::false_type());
   if (splits > 1) join_dkv_kernel<T><<<blocks_for(rows, kWaves), kThreads, 0, stream>>>(a, splits, rows, p);
 }

@@ -546,3 +546,18 @@ def test_scores_of_minus_infinity(name, dtype):
     for n, x in got["cpu"].items():
         assert torch.equal(x.isnan(), got["cuda"][n].isnan().cpu()), n
         assert n != "out" or torch.equal(x == 0, got["cuda"][n].cpu() == 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L", [3, 36, 37])
+def test_alone_and_in_a_batch(L, dtype, device):
+    """A short sequence's outputs and gradients do not depend on the others of its batch: bit for bit
+    on the GPU; on the CPU a library's products may sum in another order, some U of what they sum."""
+    q, k, v, dout, more = inputs(case(B=64 if device == "cuda" else 3, Lq=L, H=12, D=64), dtype, device)
+    batch, alone = run(q, k, v, dout, more), run(*(x[2:3] for x in (q, k, v, dout)), more)
+    _, tol = exact(*(x[2:3] for x in (q, k, v, dout)), more, dtype)
+    for n in alone:
+        if device == "cuda":
+            assert torch.equal(alone[n], batch[n][2:3]), n
+        assert_within(alone[n], batch[n][2:3], 2 * tol[n], n)
