@@ -220,6 +220,7 @@ std::vector<Tensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor frequ
   TORCH_CHECK_VALUE(P >= 1 && P <= 512 && 2 * P <= q.size(3), "rotary: ", P, " frequencies do not fit heads of ", q.size(3), " (at most 512)");
   TORCH_CHECK_TYPE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "rotary: positions are int32 or int64, got ",
                    positions.scalar_type());
+  TORCH_CHECK(!at::GradMode::is_enabled() || !frequencies.requires_grad(), "rotary: frequencies have no gradient");
   const bool axes = frequencies.dim() == 2;
   const int64_t lead = positions.dim() - axes;
   TORCH_CHECK_VALUE((lead == 1 || lead == 2) && positions.size(lead - 1) == q.size(1) && (lead == 1 || positions.size(0) == q.size(0)) &&

@@ -108,7 +108,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     differentiable in q and k.  `positions` is int32 or int64: [length] or
     [batch, length], with one more dimension of axes where `frequencies` is
     [axes, n] (axis a turns pairs a n to a n + n).  `frequencies` is fp64, from
-    `rotary_frequencies`; cosines and sines are multiplied by `amplitude`."""
+    `rotary_frequencies`, and gets no gradient; cosines and sines are multiplied by
+    `amplitude`."""
     if q.is_cuda:  # checked there, as below
         out = _backend.ext().rotary(q, k, positions, frequencies, interleaved, amplitude)
         return out[0] if k is None else tuple(out)
@@ -123,6 +124,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             raise ValueError(f"rotary: q {tuple(q.shape)} and k {tuple(x.shape)} do not go together")
     if frequencies.dtype != torch.float64 or frequencies.dim() not in (1, 2):
         raise TypeError(f"rotary: frequencies are fp64 [n] or [axes, n], got {frequencies.dtype} {tuple(frequencies.shape)}")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("rotary: frequencies have no gradient")
     P = frequencies.numel()
     if not 1 <= P <= MAX_PAIRS or 2 * P > q.shape[3]:
         raise ValueError(f"rotary: {P} frequencies do not fit heads of {q.shape[3]} (at most {MAX_PAIRS})")

@@ -162,3 +162,13 @@ def test_captured_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     for out in replays(lambda: rotary(q, k, pos, f)):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_frequencies_that_want_a_gradient_are_refused(device):
+    f = rotary_frequencies(16, device=device)[0].requires_grad_()
+    q, pos = torch.randn(1, 3, 1, 16, device=device), torch.arange(3, device=device)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rotary(q, None, pos, f)
+    with torch.no_grad():
+        assert torch.equal(rotary(q, None, pos, f), rotary(q, None, pos, f.detach()))
