@@ -214,6 +214,9 @@ std::vector<Tensor> rotary(Tensor q, OptTensor k, Tensor positions, Tensor frequ
   };
   check(q, "q");
   if (k.has_value()) check(*k, "k");
+  const int64_t heads = q.size(2) + (k.has_value() ? k->size(2) : 0);
+  TORCH_CHECK_VALUE(heads <= 4096 && q.size(3) <= 4096, "rotary: up to 4096 heads of q and k together and widths up to 4096 expected, got ", heads,
+                    " of ", q.size(3));
   TORCH_CHECK_TYPE(frequencies.scalar_type() == at::kDouble && (frequencies.dim() == 1 || frequencies.dim() == 2),
                    "rotary: frequencies are fp64 [n] or [axes, n], got ", frequencies.scalar_type(), " ", frequencies.sizes());
   const int64_t P = frequencies.numel();

@@ -42,10 +42,10 @@ struct RotaryArgs {
   Strides qs, ks;
   const void* pos; bool pos64; int64_t pb, pl, pa;
   const double* freq;
-  int n, P, D, Hq, H, tokens_per_block;  // H: heads of q and k together
+  int n, P, D, Hq, H, tokens_per_block, heads_per_block;  // H: heads of q and k together
   int64_t tokens, L;
   float amplitude, sign;
-  Divider per_head, heads;  // items of a head; heads of a token
+  Divider per_head, heads;  // items of a head; heads of a token in a block
 };
 
 // One rounding fewer than two products and a sum, and the same in every variant.
@@ -79,12 +79,13 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 
   constexpr int W = VEC ? 8 : 1;
   const int rot_items = a.P / W;
-  const int items = count * a.H * a.per_head.d;
+  const int items = count * a.heads_per_block * a.per_head.d;
   for (int i = threadIdx.x; i < items; i += kThreads) {
     const int th = a.per_head.quotient(i);   // token and head
     const int c = i - th * a.per_head.d;
     const int j = a.heads.quotient(th);
-    const int h = th - j * a.H;
+    const int h = blockIdx.y * a.heads_per_block + th - j * a.heads_per_block;
+    if (h >= a.H) break;  // the last heads' blocks hold one token each
     const bool is_q = h < a.Hq;
     const T* src = is_q ? static_cast<const T*>(a.q) + q_at[j] + h * a.qs.h
                         : static_cast<const T*>(a.k) + k_at[j] + (h - a.Hq) * a.ks.h;
@@ -163,7 +164,7 @@ std::vector<torch::Tensor> rotary_turn(torch::Tensor q, c10::optional<torch::Ten
                   positions.size(1) == L && positions.size(2) >= 1 && P % positions.size(2) == 0 &&
                   (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong),
               "rotary: positions are int32 or int64 [batch, length, axes]");
-  TORCH_CHECK(D <= 4096 && Hq + Hk <= 4096, "rotary: heads too many or too wide");
+  TORCH_CHECK(D <= 4096 && Hq + Hk <= 4096, "rotary: heads too many or too wide");  // and per_head, at most D, under 2^16
   at::DeviceGuard guard(q.device());
   auto qo = torch::empty({B, L, Hq, D}, q.options());
   auto ko = k.has_value() ? torch::empty({B, L, Hk, D}, q.options()) : torch::Tensor();
@@ -175,12 +176,13 @@ std::vector<torch::Tensor> rotary_turn(torch::Tensor q, c10::optional<torch::Ten
   const int64_t per_head = vec ? P / 8 + (D - 2 * P) / 8 : P + (D - 2 * P);
   // as many tokens as fill the table's 256 threads, fewer where that leaves CUs
   // without work, and items that stay under the divider's 2^16
+  const int64_t block_heads = std::min<int64_t>(H, 65535 / per_head);  // a token's heads go over blocks where they are more
   int64_t per_block = std::min<int64_t>({kThreads / std::min<int64_t>(P, kThreads), kMaxTokens,
-                                         (tokens + 511) / 512, 65535 / (H * per_head)});
-  per_block = std::max<int64_t>(per_block, 1);
-  TORCH_CHECK(H * per_head < 65536, "rotary: over 65535 items a token");
-  const int64_t grid = (tokens + per_block - 1) / per_block;
-  TORCH_CHECK(grid < (int64_t{1} << 31), "rotary: too many tokens");
+                                         (tokens + 511) / 512, 65535 / (block_heads * per_head)});
+  per_block = block_heads < H ? 1 : std::max<int64_t>(per_block, 1);
+  const int64_t blocks = (tokens + per_block - 1) / per_block;
+  TORCH_CHECK(blocks < (int64_t{1} << 31), "rotary: too many tokens");
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((H + block_heads - 1) / block_heads));
   RotaryArgs a{q.data_ptr(), k.has_value() ? k->data_ptr() : nullptr, qo.data_ptr(),
                k.has_value() ? ko.data_ptr() : nullptr,
                Strides{q.stride(0), q.stride(1), q.stride(2)},
@@ -189,8 +191,8 @@ std::vector<torch::Tensor> rotary_turn(torch::Tensor q, c10::optional<torch::Ten
                positions.stride(0), positions.stride(1), positions.stride(2),
                frequencies.data_ptr<double>(), static_cast<int>(P / positions.size(2)),
                static_cast<int>(P), static_cast<int>(D), static_cast<int>(Hq), static_cast<int>(H),
-               static_cast<int>(per_block), tokens, L, static_cast<float>(amplitude),
-               backward ? -1.f : 1.f, Divider(per_head), Divider(H)};
+               static_cast<int>(per_block), static_cast<int>(block_heads), tokens, L, static_cast<float>(amplitude),
+               backward ? -1.f : 1.f, Divider(per_head), Divider(block_heads)};
   auto stream = at::hip::getCurrentHIPStream();
   DISPATCH_FLOAT(q.scalar_type(), "rotary", [&] {
     if (vec) {

@@ -21,6 +21,7 @@ from . import _backend
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 MAX_PAIRS = 512
+MAX_HEADS = MAX_WIDTH = 4096  # heads of q and k together
 SCALINGS = (None, "linear", "base", "ramp")
 
 
@@ -105,7 +106,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
            interleaved: bool = False, amplitude: float = 1.0) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """q [batch, length, heads, width], and k with heads of its own (or None), with
     the first 2 * frequencies.numel() elements of every head turned; contiguous,
-    differentiable in q and k.  `positions` is int32 or int64: [length] or
+    differentiable in q and k.  Up to 4096 heads of both together, widths up to 4096,
+    512 frequencies.  `positions` is int32 or int64: [length] or
     [batch, length], with one more dimension of axes where `frequencies` is
     [axes, n] (axis a turns pairs a n to a n + n).  `frequencies` is fp64, from
     `rotary_frequencies`, and gets no gradient; cosines and sines are multiplied by
@@ -122,6 +124,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
             raise TypeError(f"rotary: q and k are fp32, bf16 or fp16 of one type, got {name} {x.dtype}")
         if x.shape[:2] != q.shape[:2] or x.shape[3] != q.shape[3]:
             raise ValueError(f"rotary: q {tuple(q.shape)} and k {tuple(x.shape)} do not go together")
+    heads = q.shape[2] + (0 if k is None else k.shape[2])
+    if heads > MAX_HEADS or q.shape[3] > MAX_WIDTH:
+        raise ValueError(f"rotary: up to {MAX_HEADS} heads of q and k together and widths up to {MAX_WIDTH} expected, got {heads} of {q.shape[3]}")
     if frequencies.dtype != torch.float64 or frequencies.dim() not in (1, 2):
         raise TypeError(f"rotary: frequencies are fp64 [n] or [axes, n], got {frequencies.dtype} {tuple(frequencies.shape)}")
     if frequencies.requires_grad and torch.is_grad_enabled():

@@ -172,3 +172,28 @@ def test_frequencies_that_want_a_gradient_are_refused(device):
         rotary(q, None, pos, f)
     with torch.no_grad():
         assert torch.equal(rotary(q, None, pos, f), rotary(q, None, pos, f.detach()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("heads,shift", [(4000, 0), (4000, 1), (1366, 1)])
+def test_many_heads(heads, shift, device):
+    """More items a token than one workgroup counts, by ones (rows off the 16-byte border) and by
+    eights: each head as in a call of its own."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(shift + 2 * heads * 64, generator=g).to(device)[shift:].view(1, 2, heads, 64)
+    k = torch.randn(1, 2, 96, 64, generator=g).to(device)
+    f, pos = rotary_frequencies(32, device=device)[0], torch.tensor([3, 70], device=device)
+    q_out, k_out = rotary(x, k, pos, f)
+    parts = [rotary(x[:, :, a:a + 50], None, pos, f) for a in range(0, heads, 50)]
+    assert torch.equal(q_out, torch.cat(parts, 2)) and torch.equal(k_out, rotary(k, None, pos, f))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refused_sizes(device):
+    f, pos = rotary_frequencies(8, device=device)[0], torch.arange(1, device=device)
+    zeros = lambda *s: torch.zeros(*s, device=device)  # noqa: E731
+    for q, k in ((zeros(1, 1, 1, 4104), None), (zeros(1, 1, 4097, 8), None), (zeros(1, 1, 4000, 8), zeros(1, 1, 97, 8))):
+        with pytest.raises(ValueError):
+            rotary(q, k, pos, f)
+    assert rotary(zeros(1, 1, 4000, 8), zeros(1, 1, 96, 8), pos, f)[0].shape == (1, 1, 4000, 8)
+    assert rotary(zeros(1, 1, 1, 4096), None, pos, f).shape == (1, 1, 1, 4096)
