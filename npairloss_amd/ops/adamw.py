@@ -83,6 +83,10 @@ def _check(params, grads, exp_avgs, exp_avg_sqs, steps, masters, scales) -> List
                                    or scales[i].device != device or not scales[i].is_contiguous()):
             raise ValueError(f"adamw_step: scales {i} {tuple(scales[i].shape)} are not fp32 [blocks of {BLOCK}, 2]")
         laid.append(g if _like(g, p) else torch.empty_like(p).copy_(g))
+    written = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
+                     for xs in (params, exp_avgs, exp_avg_sqs, steps, masters or (), scales or ()) for x in xs if x.numel())
+    if any(a[1] > b[0] for a, b in zip(written, written[1:])):
+        raise RuntimeError("adamw_step: a tensor comes twice, or overlaps another")
     return laid
 
 
@@ -94,7 +98,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     """Updates every list in place; state as `adamw_state` makes it.
 
     The parameters are of one type on one device and dense in memory, a gradient
-    of its parameter's type; one that lies in another order is copied first.
+    of its parameter's type; one that lies in another order is copied first.  What is
+    updated comes once: tensors that share memory are refused, steps too.
     `steps` counts the steps done, one int32 on the device a tensor, read and
     raised there (a captured step counts on).  With `masters` (fp32) they are
     updated and the parameters rounded from them; with `scales` the moments are

@@ -35,6 +35,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "vec.h"
 
@@ -324,12 +325,16 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
     TORCH_CHECK_VALUE(n < (int64_t{1} << 40), "adamw_step: parameter ", i, " is too large");
   }
   const auto lists = {&params, &ms, &vs, &steps, &masters, &scales};
-  std::vector<const void*> written;  // what comes twice would be updated by two workgroups at once
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // what comes twice would be updated by two workgroups at once
   for (const auto* list : lists)
     for (const auto& x : *list)
-      if (x.numel() > 0) written.push_back(x.data_ptr());
+      if (x.numel() > 0) {
+        const auto begin = reinterpret_cast<uintptr_t>(x.data_ptr());
+        written.emplace_back(begin, begin + x.numel() * x.element_size());
+      }
   std::sort(written.begin(), written.end());
-  TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), "adamw_step: a tensor comes twice");
+  for (size_t i = 1; i < written.size(); ++i)
+    TORCH_CHECK(written[i - 1].second <= written[i].first, "adamw_step: a tensor comes twice, or overlaps another");
   for (const auto* list : lists)  // a graph that has saved one of them learns of the change
     for (const auto& x : *list) x.unsafeGetTensorImpl()->bump_version();
   at::DeviceGuard guard(device);

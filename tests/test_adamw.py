@@ -346,3 +346,23 @@ def test_hash_is_even():
             c = u - 0.5
             for a, b in ((c[:, 1:], c[:, :-1]), (c[1:], c[:-1])):
                 assert abs(float((a * b).mean())) < 6 / (12 * math.sqrt(n))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["param", "exp_avg", "exp_avg_sq", "step", "part"])
+def test_what_shares_memory_is_refused(which, device):
+    """Whole or in part, before anything is changed."""
+    params, grads, states = make([(300,), (300,)], torch.float32, device, 32, False)
+    if which == "param":
+        params[1] = params[0]
+    elif which == "part":
+        both = torch.randn(500, device=device)
+        params = [both[:300], both[200:]]
+    else:
+        states[1][which] = states[0][which]
+    before = [p.clone() for p in params]
+    with pytest.raises(RuntimeError, match="twice"):
+        call(params, grads, states)
+    assert all(torch.equal(a, b) for a, b in zip(params, before)) and int(states[0]["step"]) == 0
+    both = torch.randn(600, device=device)
+    call([both[:300], both[300:]], *make([(300,), (300,)], torch.float32, device, 32, False)[1:])
