@@ -119,7 +119,8 @@ class RotaryViTB16(nn.Module):
 
     def _turns(self, device: torch.device) -> Tuple[torch.Tensor, float]:
         if device not in self._frequencies:
-            self._frequencies[device] = self._frequencies[None].to(device)
+            with torch.inference_mode(False):  # training may come after: it cannot save what inference mode made
+                self._frequencies[device] = self._frequencies[None].to(device)
         return self._frequencies[device], self.amplitude
 
     def _patches(self, image: torch.Tensor) -> torch.Tensor:

@@ -190,3 +190,18 @@ def test_bf16_autocast():
     near(got, want.detach().double().cpu(), 30 * 2.0 ** -8, "autocast")
     got.float().square().mean().backward()
     assert all(p.grad is not None and p.grad.isfinite().all() and p.grad.dtype == torch.float32 for p in m.parameters())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_training_after_inference_mode(device):
+    """What a model keeps of its first pass, in inference mode, serves a training pass."""
+    m, other = model_of(device), model_of(device)
+    x = torch.randn(2, 3, 8, 12, generator=torch.Generator().manual_seed(4)).to(device)
+    with torch.inference_mode():
+        first = m(x).clone()
+    out = m(x)
+    assert torch.equal(out, first)
+    out.sum().backward()
+    other(x).sum().backward()
+    for (n, p), q in zip(m.named_parameters(), other.named_parameters()):
+        near(p.grad, q[1].grad.double().cpu(), BACKWARD, n)
