@@ -561,3 +561,50 @@ def test_alone_and_in_a_batch(L, dtype, device):
         if device == "cuda":
             assert torch.equal(alone[n], batch[n][2:3]), n
         assert_within(alone[n], batch[n][2:3], 2 * tol[n], n)
+
+
+MANY_TILES = {
+    "plain": case(B=2, Lq=520, H=16, D=64),
+    "uneven, causal, prefix, slopes": case(B=2, Lq=390, Lk=600, H=20, D=128, causal=True, prefix=[90, 0], slopes=True),
+    "documents, capped": case(B=2, Lq=520, H=16, D=64, documents="packed", softcap=20.0),
+    "documents, capped, slopes, causal": case(B=2, Lq=520, H=32, Hk=8, D=128, documents="mixed", softcap=20.0, slopes=True, causal=True),
+    "width 80": case(B=2, Lq=520, H=16, D=80, causal=True),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", MANY_TILES)
+def test_formula_of_many_tiles(name, dtype):
+    """Heads and rows enough (512 groups of 32 queries) for tiles of 128 queries over more than 384
+    keys, forward and backward, in every type and at both padded widths.
+
+    A distance bias of 1/2 a place leaves keys that only queries 175 places on see, with weights
+    under 2^-126, the least normal fp32, which exponentials and products may give as zero.  Each
+    weight is then off by up to 2^-126, each score gradient by that times its factors (|dP| and
+    |delta|, both at most the largest sum of |dO| |V|, and the scale), each product by 2^-126."""
+    q, k, v, dout, more = inputs(MANY_TILES[name], dtype, "cuda")
+    got = run(q, k, v, dout, more)
+    want, tol = exact(q, k, v, dout, more, dtype)
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    top = lambda x: float(x.abs().max())  # noqa: E731
+    both = 2 * D * top(dout) * top(v) * D ** -0.5
+    flushed = {"out": Lk * (top(v) + 1), "dq": Lk * (both * top(k) + 1), "dk": Lq * H // Hk * (both * top(q) + 1), "dv": Lq * H // Hk * (top(dout) + 1)}
+    for n in want:
+        assert_within(got[n], want[n], tol[n] + 2.0 ** -126 * flushed[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["documents, causal", "uneven", "few queries, long"])
+def test_captured_fp16(name):
+    """The factors of fp16's score gradients are made anew at every replay, from what the gradient
+    then holds."""
+    q, k, v, dout, more = inputs(CASES[name], torch.float16, "cuda")
+    other = dout * 64
+    want = {1: run(q, k, v, dout, more), 64: run(q, k, v, other, more)}
+    by = 1
+    for out in replays(lambda: run(q, k, v, dout, more), 4):
+        assert all(torch.equal(out[n], want[by][n]) for n in out), by
+        by = 65 - by
+        dout.mul_(64 if by == 64 else 1 / 64)
