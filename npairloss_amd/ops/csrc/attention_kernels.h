@@ -274,7 +274,7 @@ DEVINL bool repairs(const AttnArgs& a) { return std::is_same<T, fp16_t>::value |
 // workgroups of width 64 a CU (two of 128).  Bound by the vector units at width 64 (an
 // exponential and seven more instructions a score; 48% of the time, products 15%), which a
 // wave's waits leave idle, and by the products at width 128.  64 images of 197 tokens, 12
-// heads of 64 bf16: 37 us; 8191 tokens, 16 heads of 128 fp16, causal: 390 us, 705 TFLOP/s.
+// heads of 64 bf16: 36 us; 8191 tokens, 16 heads of 128 fp16, causal: 371 us, 744 TFLOP/s.
 template <typename T, int DP, Score SC>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void forward_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
   constexpr int KT = sizeof(T) == 2 ? 64 : 32, NS = KT / 32;
@@ -591,8 +591,8 @@ __global__ __launch_bounds__(kThreads) void join_splits_kernel(AttnArgs a, int s
 //   P^T = 2^(S^T - lse), dS^T = P^T (V dO^T - delta) bend, dQ^T += K^T dS^T
 // A kernel of its own and not sums of dK's workgroups into dQ: those would have to be atomic,
 // in an order that changes, or another pass.  It costs two of seven products.  64 images of
-// 197 tokens, 12 heads of 64 bf16: 47 us; 8191 tokens, 16 heads of 128 fp16, causal: 460 us,
-// 900 TFLOP/s, of 1087 in a large library product.
+// 197 tokens, 12 heads of 64 bf16: 46 us; 8191 tokens, 16 heads of 128 fp16, causal: 427 us,
+// 969 TFLOP/s, of 1091 in a large library product.
 template <typename T, int DP, Score SC, bool FINE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_kernel(AttnArgs a, const DocRange* ranges, int q_tiles) {
   constexpr int KT = sizeof(T) == 2 && DP == 64 ? 64 : 32;
@@ -617,8 +617,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
     for (int x = 0; x < DP / 16; ++x) qf[x].v = -qf[x].v;
   }
   // delta = sum_d dO o, with what o's rounding left: it is subtracted from every dP of a
-  // row, so that its error does not average out, and with o in 16 bits it was the
-  // largest in dQ and dK.
+  // row, so that its error does not average out.  With o in 16 bits dQ and dK of short rows
+  // are further off: 2.27 times as far as by their own rounding with 2 keys a row, where they
+  // are 1.53 with the rest, 1.80 : 1.49 with 4, 1.56 : 1.47 with 16, 1.44 : 1.42 with 197, in
+  // bf16 and fp16 alike.  Rows of packed documents are that short in long calls too.
   float delta = 0.f, high = 0.f;
   {
     const int64_t row = ((static_cast<int64_t>(b) * a.Lq + (ok ? i : 0)) * a.H + h) * a.D;
@@ -820,8 +822,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dq_tiles_ker
 //   P = 2^(S - lse), dV^T += dO^T P, dS = P (dO V^T - delta) bend, dK^T += Q^T dS
 // Bound by registers: both sums, and K's and V's operands, are 192 of a wave's 256 at width
 // 128, and what is left sets how far reads and weights go ahead of the products.  64 images of
-// 197 tokens, 12 heads of 64 bf16: 53 us; 8191 tokens, 16 heads on 4 of 128 fp16, causal:
-// 790 us, 700 TFLOP/s, of 1087 in a large library product, and 60 us for the join of eight
+// 197 tokens, 12 heads of 64 bf16: 51 us; 8191 tokens, 16 heads on 4 of 128 fp16, causal:
+// 706 us, 782 TFLOP/s, of 1091 in a large library product, and 55 us for the join of eight
 // parts (4.5 TB/s).
 template <typename T, int DP, Score SC, bool FINE>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_tiles_kernel(AttnArgs a, const DocRange* ranges, int k_blocks, int splits, float* __restrict__ part) {
