@@ -45,6 +45,7 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 4096;
 constexpr int kBlock = 256;    // elements to a scale
 constexpr int kTensors = 52;   // of a launch: its arguments stay under 4 KB
+constexpr int kMostChunks = 1 << 23;  // of a launch: under 2^32 threads
 constexpr int kSteps = 400;    // of a launch that raises counts
 constexpr float kFp8Max = 448.f;
 constexpr float kInvMax = 1.f / 448.f;
@@ -322,7 +323,7 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
                                  scales[i].dim() == 2 && scales[i].size(0) == (n + kBlock - 1) / kBlock && scales[i].size(1) == 2 &&
                                  reinterpret_cast<uintptr_t>(scales[i].data_ptr()) % 8 == 0),
                       "adamw_step: scales ", i, " are not fp32 [blocks of ", kBlock, ", 2]");
-    TORCH_CHECK_VALUE(n < (int64_t{1} << 40), "adamw_step: parameter ", i, " is too large");
+    TORCH_CHECK_VALUE(n <= int64_t{kMostChunks} * kChunk, "adamw_step: parameter ", i, " is too large");
   }
   const auto lists = {&params, &ms, &vs, &steps, &masters, &scales};
   std::vector<std::pair<uintptr_t, uintptr_t>> written;  // what comes twice would be updated by two workgroups at once
@@ -369,7 +370,7 @@ void adamw_update(std::vector<torch::Tensor> params, std::vector<torch::Tensor> 
   a.index0 = 0;
   for (size_t i = 0; i < count; ++i) {
     const int64_t n = params[i].numel(), more = (n + kChunk - 1) / kChunk;
-    if (a.count == kTensors || (a.count > 0 && chunks + more > (1 << 30))) flush(i);
+    if (a.count == kTensors || (a.count > 0 && chunks + more > kMostChunks)) flush(i);
     a.t[a.count] = Tensor{params[i].data_ptr(), grads[i].data_ptr(), ms[i].data_ptr(), vs[i].data_ptr(),
                           masters.empty() ? nullptr : masters[i].data_ptr<float>(),
                           eight ? scales[i].data_ptr<float>() : nullptr, steps[i].data_ptr<int>(), n};

@@ -69,7 +69,7 @@ DEVINL float suffix_max(float v) {
 // keys see go by maxima of 32; in other tiles of 64 lanes are first queries, for each id a
 // maximum over those behind every lane, then keys, which take theirs.  8191 tokens, 16 heads on
 // 4, causal: 7 us, by rows and not blocks of 32 it was 40; two rows of 4096 packed with images,
-// 12 heads: 12 us. 
+// 12 heads: 12 us.
 constexpr int kLiftWaves = 4, kLiftRuns = 8;
 
 __global__ __launch_bounds__(kLiftWaves * WAVE) void key_lifts_kernel(AttnArgs a, const DocRange* ranges, int key_tiles) {
@@ -197,7 +197,7 @@ torch::Tensor doc_ranges(const c10::optional<torch::Tensor>& ids, int B, int L, 
   if (!ids.has_value()) return torch::Tensor();
   const int tiles = (L + kDocTile - 1) / kDocTile;
   auto out = torch::empty({static_cast<int64_t>(B) * tiles, 4}, ids->options());
-  TORCH_CHECK(static_cast<int64_t>(B) * tiles < (int64_t{1} << 31), "attention: too many rows");
+  TORCH_CHECK(launchable(static_cast<int64_t>(B) * tiles, WAVE), "attention: too many rows");
   doc_ranges_kernel<<<B * tiles, WAVE, 0, stream>>>(
       ids->data_ptr<int>(), L, tiles, reinterpret_cast<DocRange*>(out.data_ptr<int>()));
   HIP_CHECK_LAST();
@@ -212,7 +212,7 @@ const DocRange* ranges_of(const torch::Tensor& x) {
 // they even out by themselves.
 torch::Tensor block_order(const torch::Tensor& own, int own_rows, const torch::Tensor& other, int other_rows, int B, hipStream_t stream) {
   const int blocks = (own_rows + kBlockRows - 1) / kBlockRows;
-  if (!own.defined() || blocks < 2 || blocks > kMostOrdered) return torch::Tensor();
+  if (!own.defined() || blocks < 2 || blocks > kMostOrdered || !launchable(B, kMostOrdered)) return torch::Tensor();
   auto out = torch::empty({B, blocks}, own.options());
   block_order_kernel<<<B, (blocks + WAVE - 1) / WAVE * WAVE, 0, stream>>>(
       ranges_of(own), (own_rows + kDocTile - 1) / kDocTile, ranges_of(other), (other_rows + kDocTile - 1) / kDocTile, blocks, out.data_ptr<int>());
@@ -236,7 +236,7 @@ struct Ranges {
 void key_lifts(const AttnArgs& a, const DocRange* q_ranges, hipStream_t stream) {
   const int key_tiles = (a.Lk + WAVE - 1) / WAVE;
   const int64_t blocks = static_cast<int64_t>(a.B) * a.Hk * key_tiles;
-  TORCH_CHECK(blocks < (int64_t{1} << 31), "attention: too many rows");
+  TORCH_CHECK(launchable(blocks, kLiftWaves * WAVE), "attention: too many rows");
   key_lifts_kernel<<<blocks, kLiftWaves * WAVE, 0, stream>>>(a, q_ranges, key_tiles);
   HIP_CHECK_LAST();
 }

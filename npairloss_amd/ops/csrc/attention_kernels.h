@@ -1144,7 +1144,7 @@ __global__ __launch_bounds__(kThreads) void join_dkv_kernel(AttnArgs a, int spli
 
 int blocks_for(int64_t items, int64_t each) {
   const int64_t n = (items + each - 1) / each;
-  TORCH_CHECK(n < (int64_t{1} << 31), "attention: too many rows");
+  TORCH_CHECK(launchable(n, kThreads), "attention: too many rows");
   return static_cast<int>(n);
 }
 

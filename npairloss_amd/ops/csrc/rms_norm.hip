@@ -106,7 +106,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd_kernel(
   constexpr int kThreads = TPR > 256 ? TPR : 256;
   __shared__ float scratch[kThreads / WAVE];
   const int t = threadIdx.x % TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / TPR) + threadIdx.x / TPR;
+  const int64_t row = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * (kThreads / TPR) + threadIdx.x / TPR;
   if (row >= N) return;  // whole waves; with TPR > 64 there is one row a block
   const int64_t at = row * D;
 
@@ -356,7 +356,8 @@ std::vector<torch::Tensor> rms_norm_fwd(torch::Tensor x, torch::Tensor weight,
       with_width<FP8>(D, [&](auto tpr, auto nch) {
         constexpr int TPR = decltype(tpr)::value, NCH = decltype(nch)::value;
         constexpr int kThreads = TPR > 256 ? TPR : 256;
-        const int grid = static_cast<int>((N + kThreads / TPR - 1) / (kThreads / TPR));
+        const int64_t blocks = (N + kThreads / TPR - 1) / (kThreads / TPR), across = std::min<int64_t>(blocks, (int64_t{1} << 31) / kThreads);
+        const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>((blocks + across - 1) / across));
         auto launch = [&](auto kernel) {
           kernel<<<grid, kThreads, 0, stream>>>(
               static_cast<const T*>(x.data_ptr()), static_cast<const T*>(r), weight.data_ptr(), w_f32,

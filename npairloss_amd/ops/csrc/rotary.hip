@@ -181,7 +181,7 @@ std::vector<torch::Tensor> rotary_turn(torch::Tensor q, c10::optional<torch::Ten
                                          (tokens + 511) / 512, 65535 / (block_heads * per_head)});
   per_block = block_heads < H ? 1 : std::max<int64_t>(per_block, 1);
   const int64_t blocks = (tokens + per_block - 1) / per_block;
-  TORCH_CHECK(blocks < (int64_t{1} << 31), "rotary: too many tokens");
+  TORCH_CHECK(launchable(blocks, kThreads), "rotary: too many tokens, ", tokens);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((H + block_heads - 1) / block_heads));
   RotaryArgs a{q.data_ptr(), k.has_value() ? k->data_ptr() : nullptr, qo.data_ptr(),
                k.has_value() ? ko.data_ptr() : nullptr,

@@ -47,6 +47,10 @@ DEVINL uint32_t pack_fp8(float a, float b, float c, float d) {
 // The larger of two magnitudes; NaN if one of them is.
 DEVINL float max_or_nan(float a, float b) { return (a > b || a != a) ? a : b; }
 
+// Whether a launch fits: beyond 2^32 - 1 threads along x the runtime starts the rest of the
+// division, and says nothing.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads < (int64_t{1} << 32); }
+
 // Runs `fn` with a value of the element type that `dtype` names.
 #define DISPATCH_FLOAT(dtype, NAME, ...)                                   \
   [&] {                                                                    \

@@ -107,7 +107,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     """q [batch, length, heads, width], and k with heads of its own (or None), with
     the first 2 * frequencies.numel() elements of every head turned; contiguous,
     differentiable in q and k.  Up to 4096 heads of both together, widths up to 4096,
-    512 frequencies.  `positions` is int32 or int64: [length] or
+    512 frequencies (on the GPU under 2^24 blocks of up to 16 tokens).  `positions` is int32 or int64: [length] or
     [batch, length], with one more dimension of axes where `frequencies` is
     [axes, n] (axis a turns pairs a n to a n + n).  `frequencies` is fp64, from
     `rotary_frequencies`, and gets no gradient; cosines and sines are multiplied by

@@ -608,3 +608,12 @@ def test_captured_fp16(name):
         assert all(torch.equal(out[n], want[by][n]) for n in out), by
         by = 65 - by
         dout.mul_(64 if by == 64 else 1 / 64)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes():
+    """2^24 tiles of 256 threads are 2^32, which a launch does not take: refused, and not cut short."""
+    x = torch.ones(2 ** 24, 1, 1, 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="too many rows"):
+        attention(x, x, x)
+    assert (attention(x[1:], x[1:], x[1:]) == 1).all()

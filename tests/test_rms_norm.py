@@ -274,3 +274,16 @@ def test_outputs_changed_in_place(shape, device):
     assert torch.equal(s.detach(), x + r + 1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward(x)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes_across():
+    """2^24 blocks of four rows are 2^32 threads, which a launch does not take along one axis."""
+    x = torch.full((2 ** 26 + 8, 8), 2.0, dtype=torch.bfloat16, device="cuda")
+    w = torch.full((8,), 3.0, dtype=torch.bfloat16, device="cuda")
+    y = rms_norm(x, w)
+    assert (y == 3).all()
+    del y
+    codes, scales = rms_norm_fp8(x, w)
+    assert (codes.view(torch.uint8) == 0x7E).all()  # 448: the largest of its row
+    assert_within(scales[-1], torch.tensor([3 / FP8_MAX]), 3 / FP8_MAX * (CHAIN + U))

@@ -197,3 +197,13 @@ def test_refused_sizes(device):
             rotary(q, k, pos, f)
     assert rotary(zeros(1, 1, 4000, 8), zeros(1, 1, 96, 8), pos, f)[0].shape == (1, 1, 4000, 8)
     assert rotary(zeros(1, 1, 1, 4096), None, pos, f).shape == (1, 1, 1, 4096)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_launch_takes():
+    """2^24 blocks of sixteen tokens are 2^32 threads: refused, and not cut short."""
+    f, n = rotary_frequencies(2, device="cuda")[0], 2 ** 28
+    q, pos = torch.ones(1, n, 1, 2, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="too many tokens"):
+        rotary(q, None, pos, f)
+    assert (rotary(q[:, 16:], None, pos[16:], f) == 1).all()
