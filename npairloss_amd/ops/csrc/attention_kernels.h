@@ -1214,12 +1214,12 @@ void run_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q
   // fp16 score gradients of rows of one tile are multiplied twice, once for what rounding took
   // from them.  Without it dQ and dK are the further off the fewer keys a row has: 1.50 times
   // as far as by the result's own rounding with 2 to 4, 1.45 with 16, 1.42 from 64 on; with it
-  // 1.15 and less.  It costs more where products are the longer part, which rows of one tile,
-  // loaded for 128 queries and keys, do not have: 64 rows of 32 tokens, 12 heads of 64, dQ and
-  // dK, dV 16.0 + 15.2 us, in bf16, with one product and no scaled gradients, 13.6 + 13.5.
+  // 1.15 and less.  A row of one tile passes under its loads and launches either way: 64 rows
+  // of 64 tokens, 12 heads of 64, dQ and dK, dV 18.8 + 17.8 us with it, 19.0 + 17.7 without; of
+  // 128 29.6 + 30.0 : 28.8 + 29.3.  In long rows it would be a quarter more products.
   bool done = false;
   if constexpr (std::is_same<T, fp16_t>::value)
-    if (a.Lq <= 32 && a.Lk <= 32) launch(std::true_type()), done = true;
+    if (a.Lq <= kDocTile && a.Lk <= kDocTile) launch(std::true_type()), done = true;
   if (!done) launch(std::false_type());
   if (splits > 1) join_dkv_kernel<T><<<blocks_for(rows, kWaves), kThreads, 0, stream>>>(a, splits, rows, p);
 }
