@@ -293,14 +293,13 @@ std::vector<torch::Tensor> attention_bwd(torch::Tensor dout, torch::Tensor q, to
   const auto k_order = one ? q_order : block_order(ranges.k, a.Lk, ranges.q, a.Lq, a.B, stream);
   a.q_order = order_of(q_order);
   a.k_order = order_of(k_order);
-  torch::Tensor tops, blocks, lifts;
+  torch::Tensor tops;  // of rows, blocks and keys, one behind another
   if (q.scalar_type() == at::kHalf) {
-    tops = torch::empty_like(lse);
-    blocks = torch::empty({a.B, a.H, (a.Lq + 31) / 32}, lse.options());
-    lifts = torch::empty({a.B, a.Hk, a.Lk}, lse.options());
+    const int64_t heads = static_cast<int64_t>(a.B) * a.H, blocks = heads * ((a.Lq + 31) / 32);
+    tops = torch::empty({heads * a.Lq + blocks + static_cast<int64_t>(a.B) * a.Hk * a.Lk}, lse.options());
     a.row_top = tops.data_ptr<float>();
-    a.block_top = blocks.data_ptr<float>();
-    a.key_lift = lifts.data_ptr<float>();
+    a.block_top = a.row_top + heads * a.Lq;
+    a.key_lift = a.block_top + blocks;
   }
   DISPATCH_FLOAT(q.scalar_type(), "attention", [&] {
     attention_backward<T>(a, ranges_of(ranges.k), ranges_of(ranges.q), q.options(), stream);
