@@ -1211,14 +1211,14 @@ void run_backward(const AttnArgs& a, const DocRange* k_ranges, const DocRange* q
     if constexpr (std::is_same<T, fp16_t>::value) key_lifts(a, q_ranges, stream);
     dkv_tiles_kernel<T, DP, SC, decltype(fine)::value><<<blocks_for(base * splits, 1), kThreads, 0, stream>>>(a, q_ranges, k_blocks, splits, p);
   };
-  // fp16 score gradients of rows of one tile are multiplied twice, once for what rounding took
+  // 16-bit score gradients of rows of one tile are multiplied twice, once for what rounding took
   // from them.  Without it dQ and dK are the further off the fewer keys a row has: 1.50 times
   // as far as by the result's own rounding with 2 to 4, 1.45 with 16, 1.42 from 64 on; with it
   // 1.15 and less.  A row of one tile passes under its loads and launches either way: 64 rows
-  // of 64 tokens, 12 heads of 64, dQ and dK, dV 18.8 + 17.8 us with it, 19.0 + 17.7 without; of
-  // 128 29.6 + 30.0 : 28.8 + 29.3.  In long rows it would be a quarter more products.
+  // of 64 tokens, 12 heads of 64 fp16, dQ and dK, dV 18.8 + 17.8 us with it, 19.0 + 17.7
+  // without; of 128 29.6 + 30.0 : 28.8 + 29.3.  In long rows it would be a quarter more products.
   bool done = false;
-  if constexpr (std::is_same<T, fp16_t>::value)
+  if constexpr (sizeof(T) == 2)
     if (a.Lq <= kDocTile && a.Lk <= kDocTile) launch(std::true_type()), done = true;
   if (!done) launch(std::false_type());
   if (splits > 1) join_dkv_kernel<T><<<blocks_for(rows, kWaves), kThreads, 0, stream>>>(a, splits, rows, p);

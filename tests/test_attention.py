@@ -632,3 +632,15 @@ def test_short_rows_in_fp16(L, D):
     off = lambda x, n: float((x.double().cpu() - want[n]).square().mean().sqrt())  # noqa: E731
     for n in ("dq", "dk"):
         assert off(got[n], n) <= 1.2 * off(want[n].to(torch.float16), n), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L,D,slopes", [(2, 64, True), (3, 32, False), (16, 64, False), (37, 64, True), (64, 128, False)])
+def test_short_rows_in_bf16(L, D, slopes):
+    """As in fp16: score gradients are multiplied twice, and dQ and dK are off by little more than
+    by their own rounding."""
+    q, k, v, dout, more = inputs(case(B=64, Lq=L, H=12 if L < 64 else 3, D=D, slopes=slopes), torch.bfloat16, "cuda")
+    got, (want, _) = run(q, k, v, dout * 0.1, more), exact(q, k, v, dout * 0.1, more, torch.bfloat16)
+    off = lambda x, n: float((x.double().cpu() - want[n]).square().mean().sqrt())  # noqa: E731
+    for n in ("dq", "dk"):
+        assert off(got[n], n) <= 1.2 * off(want[n].to(torch.bfloat16), n), n
